@@ -179,7 +179,8 @@ int smelt_hip_pipeline_count(const smelt_hip_context *ctx);
 /* 1 = launchable, 0 = fallback slot, negative = bad index */
 int smelt_hip_pipeline_is_ready(const smelt_hip_context *ctx, uint32_t index);
 
-/* Slot buffers: makeBuffer(length:) zero-filled, SmeltRuntime.swift:922-979. */
+/* Slot buffers: makeBuffer(length:) zero-filled, SmeltRuntime.swift:922-979.  A slot allocated again at its own
+ * size keeps its memory (cleared), so captured graphs that bind it stay valid. */
 int smelt_hip_buffer_alloc(smelt_hip_context *ctx, int slot, size_t bytes);
 int smelt_hip_buffer_write(smelt_hip_context *ctx, int slot, size_t offset, const void *src,
                            size_t bytes);
@@ -253,7 +254,7 @@ int smelt_hip_benchmark_record(smelt_hip_context *ctx, const SmeltDispatchRecord
  * command buffer replay.  A graph holds what the capture resolved: device addresses of the
  * slots (cur / alt included), byte offsets and constants derived from `position` (decode) or
  * `seq_len` / `start_pos` (prefill), grids derived from seq_len.  It therefore stays valid only
- * while no slot it binds is re-allocated or re-uploaded, and replays the position it was
+ * while no slot it binds is re-allocated at another size, and replays the position it was
  * captured with: a table whose records carry position-dependent offsets or constants needs one
  * capture per position (a table of matvec / qmm records carries none).  Destroy a graph before
  * freeing the slots it names. */

@@ -1665,6 +1665,13 @@ static int alloc_slot(smelt_hip_context* ctx, int slot, size_t bytes, bool read_
     if ((size_t)slot >= ctx->slots.size()) ctx->slots.resize((size_t)slot + 1);
     SlotBuffer& s = ctx->slots[(size_t)slot];
     HIP_TRY(ctx, hipSetDevice(ctx->device));
+    if (s.ptr && s.bytes == bytes) {
+        // same size: the slot keeps its memory, so that a captured graph that binds it keeps writing to live memory
+        HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+        HIP_TRY(ctx, hipMemset(s.ptr, 0, bytes + 256));
+        s.read_only = read_only;
+        return SMELT_HIP_OK;
+    }
     if (s.ptr) {
         HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
         HIP_TRY(ctx, hipFree(s.ptr));
