@@ -188,6 +188,17 @@ int smelt_hip_buffer_read(smelt_hip_context *ctx, int slot, size_t offset, void 
                           size_t bytes);
 int smelt_hip_buffer_size(const smelt_hip_context *ctx, int slot, size_t *bytes);
 
+/* No counterpart in the reference.  Binds a slot to `bytes` of device memory that the caller owns (a cache pool, another library's
+ * tensor) instead of allocating it; the memory must be on the context's device and outlive the binding.  Such slots are
+ * taken by the serving operators (smelt_hip_compiler.h), whose kernels touch exactly the bytes their shapes name; the other
+ * kernels refuse them.  Work runs on the context's stream (smelt_hip_context_stream, a hipStream_t): it is ordered after the work
+ * of the null stream, and a caller that fills or reads the memory on other streams orders them by events.  Graphs that bind
+ * the slot hold the address it had when they were captured.
+ * smelt_hip_buffer_release waits for the stream and frees (or, when bound, forgets) what the slot names. */
+int smelt_hip_buffer_bind(smelt_hip_context *ctx, int slot, void *device_ptr, size_t bytes);
+int smelt_hip_buffer_release(smelt_hip_context *ctx, int slot);
+int smelt_hip_context_stream(smelt_hip_context *ctx, void **out_stream);
+
 /* weights.bin mapping: SmeltMetalWeightStorage.swift:220-319 maps the file into page-aligned
  * MTLBuffers and resolves logical offsets (SmeltRuntime.swift:3153-3169).  HBM is not unified
  * with host memory, so the bytes are copied once into one device allocation that becomes the

@@ -208,6 +208,88 @@ int smelt_emit_view_matvec(smelt_emitter *e, int weights_slot, const SmeltWeight
 int smelt_emit_view_gate_up_swiglu(smelt_emitter *e, int weights_slot, const SmeltWeightEntryC *gate,
                                    const SmeltWeightEntryC *up, int planes, SmeltBinding view_planes,
                                    SmeltBinding view_scales, SmeltBinding output, int batch_size);
+/* ---- serving operators: what runs between the q|k|v bank and the o projection, and behind the lm_head --------------------
+ * (No counterpart in the reference's names: its attention, rope and sampling shaders are not mirrored here.)
+ * Every value of a record but the first (`tokens` / `rows`, which resolves to seqLen when dynamic != 0) is fixed when it is
+ * emitted; lengths, positions and page tables are data in bound slots, so a captured graph follows them.  The record's grid is
+ * nominal.  The emitter runs the launch's own checks (all but the slots' sizes) and refuses what the launch would refuse.
+ *
+ * Rotary positions.  A head's first rotary_dim values are rotated by position * table[i], pair i being (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) when interleaved; the rest is copied.  cos and sin are multiplied by `amplitude`.  The table is
+ * rotary_dim / 2 doubles (radians a position); positions are int32, one a token. */
+typedef struct SmeltRope {
+    int32_t head_dim;   /* 1 .. 1024 (64, 128 or 256 where the rows go to a cache) */
+    int32_t rotary_dim; /* even, at most head_dim */
+    int32_t interleaved;
+    float amplitude;
+} SmeltRope;
+
+/* Frequencies for contexts longer than the `positions` the model was trained on, by `factor`:
+ *   PLAIN   base^(-2 i / rotary_dim)
+ *   LINEAR  all divided by factor
+ *   BASE    the base multiplied by factor^(rotary_dim / (rotary_dim - 2)): the slowest pair divided, the fastest kept
+ *   BANDS   pairs of fewer than `low` turns over `positions` divided, of more than `high` kept, linear in the turns between
+ *   PARTS   as BANDS, but linear in the pair's index between those two (rounded outwards), amplitude 0.1 ln(factor) + 1 */
+enum { SMELT_ROPE_PLAIN = 0, SMELT_ROPE_LINEAR = 1, SMELT_ROPE_BASE = 2, SMELT_ROPE_BANDS = 3, SMELT_ROPE_PARTS = 4 };
+typedef struct SmeltRopeScaling {
+    int32_t kind;
+    double base, factor, positions, low, high;
+} SmeltRopeScaling;
+/* writes rotary_dim / 2 doubles and (when not NULL) the amplitude; SMELT_HIP_ERR_INVALID_ARGUMENT for values without a meaning */
+int smelt_rope_table(const SmeltRopeScaling *scaling, int rotary_dim, double *out_table, float *out_amplitude);
+
+/* "rope_{half,interleaved}_d{D}_r{R}": `tokens` rows of `heads` heads, strides in elements (>= heads * head_dim).  Output may be the
+ * input itself (same slot, offset and stride); other overlaps are refused. */
+int smelt_emit_rope(smelt_emitter *e, const SmeltRope *rope, SmeltBinding input, SmeltBinding output,
+                    SmeltBinding positions, SmeltBinding table, int heads, int input_stride,
+                    int output_stride, int tokens, int dynamic);
+
+/* A paged cache: pages of page_size (16, 32, 64, 128, 256) tokens, keys and values apart, 16-bit.
+ *   keys    [pages][kv_heads][head_dim / 8][page_size][8]   (what the matrix cores take, a page and head contiguous)
+ *   values  [pages][kv_heads][page_size][head_dim] */
+typedef struct SmeltPagedCache {
+    SmeltBinding k, v;
+    int32_t head_dim /* 64, 128, 256 */, kv_heads, page_size, pages;
+} SmeltPagedCache;
+
+/* "paged_kv_append[_q]_{half,interleaved}_d{D}_r{R}_kv{H}_p{P}": token rows k (rotated) and v put to place slots[token] = page *
+ * page_size + offset; a negative slot, or one behind the pool, puts the token nowhere.  Tokens that name the same place leave one of
+ * them, element by element unspecified which.  With q and q_out (both or neither) the q rows are rotated in the same launch,
+ * also those of tokens without a place; q_out may be q itself.  rotary_dim 0 rotates nothing. */
+int smelt_emit_paged_kv_append(smelt_emitter *e, const SmeltRope *rope, const SmeltPagedCache *cache,
+                               SmeltBinding k, SmeltBinding v, SmeltBinding positions,
+                               SmeltBinding slots, SmeltBinding table, const SmeltBinding *q,
+                               const SmeltBinding *q_out, int q_heads, int k_stride, int v_stride,
+                               int q_stride, int q_out_stride, int tokens, int dynamic);
+
+/* "paged_attention[_shared]_d{D}_h{H}_kv{H}_p{P}": sequence s has the rows offsets[s] .. offsets[s + 1] (int32[sequences + 1],
+ * ascending from 0) of q and output ([tokens][heads * head_dim]; rows from offsets[sequences] on are left as they were) and
+ * kv_lens[s] keys of its own, its new tokens' included, on the pages of page_table[s][pages_per_sequence].  prefix_table (at most
+ * prefix_pages pages) and prefix_len (one int32) name a prefix that stands before every sequence's own keys; it is read once for
+ * all of them when they have few rows each.  The last row of a sequence is the newest key's; a row sees the keys up to its
+ * own and, with window > 0, only the last `window` of them.  A row that sees nothing is zero.  Lengths are cut to what the tables
+ * hold; keys on a page outside the pool are not seen. */
+int smelt_emit_paged_attention(smelt_emitter *e, const SmeltPagedCache *cache, SmeltBinding q,
+                               SmeltBinding page_table, SmeltBinding kv_lens, SmeltBinding offsets,
+                               SmeltBinding output, const SmeltBinding *prefix_table,
+                               const SmeltBinding *prefix_len, int prefix_pages, int heads,
+                               int q_stride, int pages_per_sequence, float scale, int window,
+                               int sequences, int tokens, int dynamic);
+
+/* "verify_drafts" / "verify_drafts_given" (draft NULL): drafted tokens against the target's probabilities.  Sequence s has the logits
+ * rows offsets[s] .. offsets[s + 1] of target (16-bit, `vocab` logits at `stride` elements): row i is what follows the i-th
+ * drafted token's prefix, so its last row has no draft.  With p = softmax(target / temperature[s]) and q = softmax(draft /
+ * temperature[s]) (draft NULL: q is 1 on the drafted token): draft x of row i is taken while u_accept[row] * q(x) < p(x).  The
+ * first one refused is replaced by a token drawn from max(p - q, 0); if all are taken one more is drawn from the last row's
+ * p.  Drawing takes the lowest token whose running sum of weights passes u_sample[s] * their total (max(p - q, 0) all zero: p's).
+ * temperature <= 0 (or not a number): a draft is taken while it is the row's largest logit (lowest token of equal ones), and
+ * that token is drawn.  A draft outside the vocabulary is refused; a NaN logit counts as -inf, +inf as the largest finite number; a row
+ * without any weight draws -1.  tokens[row]: the taken drafts, the drawn token, then -1; counts[s]: taken drafts.  Rows from
+ * offsets[sequences] on are left as they were; a sequence without rows counts 0.  At most 65535 rows and sequences. */
+int smelt_emit_verify_drafts(smelt_emitter *e, SmeltBinding target, const SmeltBinding *draft,
+                             SmeltBinding draft_tokens, SmeltBinding offsets, SmeltBinding u_accept,
+                             SmeltBinding u_sample, SmeltBinding temperature, SmeltBinding tokens,
+                             SmeltBinding counts, int rows, int sequences, int vocab, int stride);
 /* swap cur/alt (SmeltDispatchRecord.swap) */
 int smelt_emit_swap(smelt_emitter *e);
 

@@ -20,14 +20,15 @@ HSACO = os.path.join(LIB, "smelt_kernels.hsaco")
 # every translation unit under csrc/kernels becomes one code object; the runtime loads them all
 KERNEL_UNITS = ["smelt_kernels", "smelt_kernels_batched_f16", "smelt_kernels_batched_bf16",
                 "smelt_kernels_signed", "smelt_kernels_planes", "smelt_kernels_qmm",
-                "smelt_kernels_layer", "smelt_kernels_mm1", "smelt_kernels_mm1f", "smelt_kernels_qms", "smelt_kernels_qmt"]
+                "smelt_kernels_layer", "smelt_kernels_mm1", "smelt_kernels_mm1f", "smelt_kernels_qms", "smelt_kernels_qmt",
+                "smelt_kernels_serving", "smelt_kernels_attn_f16", "smelt_kernels_attn_bf16"]
 HOST_LIB = os.path.join(LIB, "libsmelt_hip.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # packed fp32 instructions are switched off for all device code
 DEVICE_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17",
                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-HOST_SOURCES = ["runtime.cpp", "pipeline_table.cpp", "compiler.cpp", "import.cpp"]
+HOST_SOURCES = ["runtime.cpp", "pipeline_table.cpp", "compiler.cpp", "import.cpp", "serving.cpp"]
 
 
 def _run(cmd: list[str]) -> None:

@@ -43,6 +43,23 @@ class Binding(C.Structure):
     _fields_ = [("slot", C.c_int32), ("offset", C.c_uint64), ("offset_kind", C.c_uint8)]
 
 
+class Rope(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("amplitude", C.c_float)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("base", C.c_double), ("factor", C.c_double), ("positions", C.c_double),
+                ("low", C.c_double), ("high", C.c_double)]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("k", Binding), ("v", Binding), ("head_dim", C.c_int32), ("kv_heads", C.c_int32),
+                ("page_size", C.c_int32), ("pages", C.c_int32)]
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BANDS, ROPE_PARTS = range(5)
+
+
 def bind(slot: int, offset: int = 0, kind: int = 0) -> Binding:
     return Binding(slot, offset, kind)
 
@@ -89,6 +106,11 @@ def lib() -> C.CDLL:
         "smelt_emit_rms_norm_1pw": (i32, [vp, Binding, Binding, Binding, C.POINTER(Binding), i32, C.c_float, i32]),
         "smelt_emit_elementwise": (i32, [vp, i32, Binding, Binding, Binding, i32]),
         "smelt_emit_swiglu_fused": (i32, [vp, Binding, Binding, Binding, i32]),
+        "smelt_rope_table": (i32, [C.POINTER(RopeScaling), i32, C.POINTER(C.c_double), C.POINTER(C.c_float)]),
+        "smelt_emit_rope": (i32, [vp, C.POINTER(Rope)] + [Binding] * 4 + [i32] * 5),
+        "smelt_emit_paged_kv_append": (i32, [vp, C.POINTER(Rope), C.POINTER(PagedCache)] + [Binding] * 5 + [C.POINTER(Binding)] * 2 + [i32] * 7),
+        "smelt_emit_paged_attention": (i32, [vp, C.POINTER(PagedCache)] + [Binding] * 5 + [C.POINTER(Binding)] * 2 + [i32] * 4 + [C.c_float] + [i32] * 4),
+        "smelt_emit_verify_drafts": (i32, [vp, Binding, C.POINTER(Binding)] + [Binding] * 7 + [i32] * 4),
         "smelt_emitter_record_count": (sz, [vp]),
         "smelt_emitter_records": (C.POINTER(rt.DispatchRecord), [vp]),
         "smelt_emitter_pipeline_count": (sz, [vp]),
@@ -235,6 +257,17 @@ def plan_matvec(layout, rows, cols, group, nmat=1, lds_limit=160 * 1024, force=F
     return dict(zip(MATVEC_PLAN_FIELDS, out)) if rc else None
 
 
+def rope_table(rotary_dim, base=10000.0, kind=ROPE_PLAIN, factor=1.0, positions=8192.0, low=1.0, high=4.0):
+    """(radians a position of each pair as float64, amplitude) for a rotation scaled to longer contexts."""
+    out = np.zeros(max(rotary_dim // 2, 1), np.float64)
+    amplitude = C.c_float(1.0)
+    rc = lib().smelt_rope_table(C.byref(RopeScaling(kind, base, factor, positions, low, high)), rotary_dim,
+                                out.ctypes.data_as(C.POINTER(C.c_double)), C.byref(amplitude))
+    if rc != 0:
+        raise ValueError(f"smelt_rope_table: {rc}")
+    return out, float(amplitude.value)
+
+
 class EmitError(RuntimeError):
     def __init__(self, code, message):
         super().__init__(f"emit error {code}: {message}")
@@ -247,6 +280,7 @@ class Emitter:
 
     def __init__(self, act_dtype=rt.ACT_F16, compute_units=256):
         self.l = lib()
+        self.act_dtype = act_dtype
         h = C.c_void_p()
         rc = self.l.smelt_emitter_create(act_dtype, compute_units, C.byref(h))
         if rc != 0:
@@ -338,6 +372,45 @@ class Emitter:
         self._check(self.l.smelt_emit_view_gate_up_swiglu(self.h, weights_slot, C.byref(gate), C.byref(up), planes,
                                                           view_planes, view_scales, y, batch))
 
+    # -- serving operators (include/smelt_hip_compiler.h) --------------------------------------------
+    def rope(self, x, y, positions, table, tokens, heads, head_dim, rotary_dim, interleaved=False, amplitude=1.0,
+             x_stride=None, y_stride=None, dynamic=False):
+        """Rows of `heads` heads rotated to their positions; y may be x."""
+        rope = Rope(head_dim, rotary_dim, int(interleaved), amplitude)
+        row = heads * head_dim
+        self._check(self.l.smelt_emit_rope(self.h, C.byref(rope), x, y, positions, table, heads, row if x_stride is None else x_stride,
+                                           row if y_stride is None else y_stride, tokens, int(dynamic)))
+
+    def paged_kv_append(self, k, v, positions, slots, table, k_cache, v_cache, tokens, kv_heads, head_dim, rotary_dim,
+                        page_size, pages, interleaved=False, amplitude=1.0, kv_stride=None, v_stride=None, q=None,
+                        q_out=None, q_heads=0, q_stride=None, q_out_stride=None, dynamic=False):
+        """k (rotated) and v rows to their places of a paged cache; with q and q_out also q rotated."""
+        rope = Rope(head_dim, rotary_dim, int(interleaved), amplitude)
+        cache = PagedCache(k_cache, v_cache, head_dim, kv_heads, page_size, pages)
+        kv_stride = kv_heads * head_dim if kv_stride is None else kv_stride
+        row = q_heads * head_dim
+        self._check(self.l.smelt_emit_paged_kv_append(
+            self.h, C.byref(rope), C.byref(cache), k, v, positions, slots, table, None if q is None else C.byref(q),
+            None if q_out is None else C.byref(q_out), q_heads, kv_stride, kv_stride if v_stride is None else v_stride,
+            row if q_stride is None else q_stride, row if q_out_stride is None else q_out_stride, tokens, int(dynamic)))
+
+    def paged_attention(self, q, k_cache, v_cache, page_table, kv_lens, offsets, out, tokens, sequences, heads, kv_heads,
+                        head_dim, page_size, pages, pages_per_sequence, scale, window=0, q_stride=None, prefix_table=None,
+                        prefix_len=None, prefix_pages=0, dynamic=False):
+        """Attention of new token rows over their sequences' pages, behind a prefix that all of them share."""
+        cache = PagedCache(k_cache, v_cache, head_dim, kv_heads, page_size, pages)
+        self._check(self.l.smelt_emit_paged_attention(
+            self.h, C.byref(cache), q, page_table, kv_lens, offsets, out, None if prefix_table is None else C.byref(prefix_table),
+            None if prefix_len is None else C.byref(prefix_len), prefix_pages, heads, heads * head_dim if q_stride is None else q_stride,
+            pages_per_sequence, scale, window, sequences, tokens, int(dynamic)))
+
+    def verify_drafts(self, target, draft_tokens, offsets, u_accept, u_sample, temperature, tokens, counts, rows, sequences,
+                      vocab, stride=None, draft=None):
+        """Drafted tokens taken or refused against the target's logits, and the token drawn behind them."""
+        self._check(self.l.smelt_emit_verify_drafts(self.h, target, None if draft is None else C.byref(draft), draft_tokens, offsets,
+                                                    u_accept, u_sample, temperature, tokens, counts, rows, sequences, vocab,
+                                                    vocab if stride is None else stride))
+
     def swap(self):
         self._check(self.l.smelt_emit_swap(self.h))
 
@@ -357,6 +430,19 @@ class Emitter:
         if n:
             C.memmove(arr, self.l.smelt_emitter_records(self.h), n * C.sizeof(rt.DispatchRecord))
         return arr
+
+    def table_for(self, ctx: rt.Context):
+        """The records with their pipelines looked up (or created) in `ctx`, which may hold other emitters' pipelines too."""
+        index = [ctx.pipeline(self._entry(name)) for name in self.pipelines]
+        arr = self.records()
+        for r in arr:
+            if r.op_kind == 0:
+                r.pipeline = index[r.pipeline]
+        return arr
+
+    def _entry(self, name: str) -> str:
+        """A pipeline name that says the emitter's activation type, whatever the context's default is."""
+        return name if "@" in name else name + ("@bf16" if self.act_dtype == rt.ACT_BF16 else "@f16")
 
     def install(self, ctx: rt.Context) -> None:
         """Create the context's pipeline table in manifest order (index == record.pipeline)."""

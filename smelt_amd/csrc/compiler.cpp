@@ -2,6 +2,7 @@
 // shape routing and dispatch-record emitters.  Mirrors the cited parts of SmeltCompiler; the
 // launch geometry is this backend's own (256-thread workgroups, grid-stride rows).
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -9,6 +10,7 @@
 
 #include "../../include/smelt_hip_compiler.h"
 #include "pipeline_table.hpp"
+#include "serving.hpp"
 
 using namespace smelt_host;
 
@@ -1103,6 +1105,144 @@ int smelt_hip_plan_matvec(int code_layout, uint32_t rows, uint32_t cols, uint32_
     if (!smelt_host::mm1_plan((smelt_host::CodeLayout)code_layout, rows, cols, group, nmat, lds_limit, force != 0, &p)) return 0;
     out[0] = p.nl; out[1] = p.kc; out[2] = (rows + 7) / 8; out[3] = 64 * p.kc; out[4] = (uint32_t)p.lds;
     return 1;
+}
+
+// ---- serving operators ------------------------------------------------------------------------------------------------------
+
+// Emits a record of a serving pipeline after running the launch's own checks on it: buffers in argument order, then the values
+// (value `dynamic_at` resolves to seqLen when dynamic).  Slots stand in for addresses: the same slot and offset are the same memory.
+static int emit_serving(smelt_emitter* e, const std::string& name, const SmeltBinding* const* buffers, int buffer_count,
+                        const uint32_t* values, int value_count, uint32_t float_mask, bool dynamic) {
+    ResolvedPipeline r;
+    std::string why;
+    const ResolveStatus st = resolve_pipeline(name, e->act == SMELT_HIP_ACT_BF16 ? kActBF16 : kActF16, 163840, &r, &why);
+    if (st == kResolveMalformed) return efail(e, SMELT_HIP_ERR_UNSUPPORTED_GEOMETRY, why);
+    if (st != kResolveOk) return efail(e, SMELT_HIP_ERR_UNKNOWN_PIPELINE, why);
+    if ((size_t)(buffer_count + value_count) + r.appended.size() != r.kinds.size() || value_count > SMELT_MAX_CONSTANTS_PER_DISPATCH)
+        return efail(e, SMELT_HIP_ERR_BINDING_MISMATCH, "argument count of '" + name + "'");
+    ServingPlan plan;
+    uint32_t all[40] = {};
+    RecordBuilder rb;
+    for (int i = 0; i < buffer_count; ++i) {
+        // (an offset that is only known at launch says nothing about where the operand lies)
+        const uintptr_t at = buffers[i]->offset_kind == 0 ? ((uintptr_t)(buffers[i]->slot + 3) << 44) + (uintptr_t)buffers[i]->offset : (uintptr_t)(8192 + i) << 44;
+        plan.operand[i].ptr = reinterpret_cast<void*>(at);
+        rb.buffer((uint8_t)i, *buffers[i]);
+    }
+    for (int i = 0; i < value_count; ++i) {
+        all[buffer_count + i] = values[i];
+        const uint8_t kind = (float_mask >> i) & 1u ? SMELT_CONST_LITERAL_F32 : (dynamic && i == 0 ? SMELT_CONST_SEQ_LEN : SMELT_CONST_LITERAL_U32);
+        rb.constant((uint8_t)(buffer_count + i), values[i], kind);
+    }
+    for (size_t i = 0; i < r.appended.size(); ++i) all[buffer_count + value_count + i] = r.appended[i];
+    ServingDevice dev;
+    dev.compute_units = (uint32_t)std::max(1, e->compute_units);
+    dev.workspace_bytes = (size_t)64 << 20;
+    if (int rc = plan_serving(r, all, dev, &plan, &why)) return efail(e, rc, "'" + name + "': " + why);
+    rb.grid(1, 1, 1, 256);   // nominal: the launch derives its geometry from the values
+    rb.r.pipeline = e->pipeline_index(name);
+    e->records.push_back(rb.r);
+    return SMELT_HIP_OK;
+}
+
+static uint32_t float_bits(float v) { uint32_t b; memcpy(&b, &v, 4); return b; }
+static bool any_negative(std::initializer_list<int> v) { for (int x : v) if (x < 0) return true; return false; }
+
+int smelt_rope_table(const SmeltRopeScaling* scaling, int rotary_dim, double* out_table, float* out_amplitude) {
+    if (!scaling || !out_table || rotary_dim <= 0 || rotary_dim % 2 != 0 || !(scaling->base > 0.0)) return SMELT_HIP_ERR_INVALID_ARGUMENT;
+    const bool scaled = scaling->kind != SMELT_ROPE_PLAIN;
+    if (scaled && !(scaling->factor > 0.0)) return SMELT_HIP_ERR_INVALID_ARGUMENT;
+    const bool split = scaling->kind == SMELT_ROPE_BANDS || scaling->kind == SMELT_ROPE_PARTS;
+    if (split && (!(scaling->positions > 0.0) || !(scaling->low > 0.0) || !(scaling->high > scaling->low))) return SMELT_HIP_ERR_INVALID_ARGUMENT;
+    const double two_pi = 6.283185307179586476925;
+    const int half = rotary_dim / 2;
+    double base = scaling->base;
+    if (scaling->kind == SMELT_ROPE_BASE) {
+        if (rotary_dim <= 2) return SMELT_HIP_ERR_INVALID_ARGUMENT;
+        base *= std::pow(scaling->factor, (double)rotary_dim / (rotary_dim - 2));
+    }
+    // the pairs whose waves turn `high` and `low` times over the original context
+    auto pair_of = [&](double turns) { return rotary_dim * std::log(scaling->positions / (turns * two_pi)) / (2.0 * std::log(base)); };
+    double first = 0.0, last = 0.0;
+    if (scaling->kind == SMELT_ROPE_PARTS) {
+        first = std::max(std::floor(pair_of(scaling->high)), 0.0);
+        last = std::min(std::ceil(pair_of(scaling->low)), (double)(rotary_dim - 1));
+    }
+    for (int i = 0; i < half; ++i) {
+        const double f = std::pow(base, -2.0 * i / rotary_dim);
+        double keep = 1.0;   // how much of the unscaled frequency stays
+        switch (scaling->kind) {
+            case SMELT_ROPE_PLAIN: case SMELT_ROPE_BASE: break;
+            case SMELT_ROPE_LINEAR: keep = 0.0; break;
+            case SMELT_ROPE_BANDS: {
+                const double turns = scaling->positions * f / two_pi;
+                keep = std::min(1.0, std::max(0.0, (turns - scaling->low) / (scaling->high - scaling->low)));
+                break;
+            }
+            case SMELT_ROPE_PARTS: keep = 1.0 - std::min(1.0, std::max(0.0, (i - first) / std::max(last - first, 0.001))); break;
+            default: return SMELT_HIP_ERR_INVALID_ARGUMENT;
+        }
+        out_table[i] = keep == 1.0 ? f : keep * f + (1.0 - keep) * f / scaling->factor;
+    }
+    if (out_amplitude) *out_amplitude = scaling->kind == SMELT_ROPE_PARTS && scaling->factor > 1.0 ? (float)(0.1 * std::log(scaling->factor) + 1.0) : 1.0f;
+    return SMELT_HIP_OK;
+}
+
+static std::string rope_tail(const SmeltRope* rope) {
+    return std::string(rope->interleaved ? "_interleaved" : "_half") + "_d" + std::to_string(rope->head_dim) + "_r" + std::to_string(rope->rotary_dim);
+}
+
+int smelt_emit_rope(smelt_emitter* e, const SmeltRope* rope, SmeltBinding input, SmeltBinding output, SmeltBinding positions, SmeltBinding table,
+                    int heads, int input_stride, int output_stride, int tokens, int dynamic) {
+    if (!e) return SMELT_HIP_ERR_INVALID_ARGUMENT;
+    if (!rope || any_negative({rope->head_dim, rope->rotary_dim, heads, input_stride, output_stride, tokens})) return efail(e, SMELT_HIP_ERR_INVALID_ARGUMENT, "rope: null shape or negative size");
+    const SmeltBinding* b[] = {&input, &output, &positions, &table};
+    const uint32_t v[] = {(uint32_t)tokens, (uint32_t)heads, (uint32_t)input_stride, (uint32_t)output_stride, float_bits(rope->amplitude)};
+    return emit_serving(e, "rope" + rope_tail(rope), b, 4, v, 5, 1u << 4, dynamic != 0);
+}
+
+int smelt_emit_paged_kv_append(smelt_emitter* e, const SmeltRope* rope, const SmeltPagedCache* cache, SmeltBinding k, SmeltBinding v, SmeltBinding positions,
+                               SmeltBinding slots, SmeltBinding table, const SmeltBinding* q, const SmeltBinding* q_out, int q_heads, int k_stride,
+                               int v_stride, int q_stride, int q_out_stride, int tokens, int dynamic) {
+    if (!e) return SMELT_HIP_ERR_INVALID_ARGUMENT;
+    if (!rope || !cache || (q == nullptr) != (q_out == nullptr) ||
+        any_negative({rope->head_dim, rope->rotary_dim, cache->kv_heads, cache->page_size, cache->pages, q_heads, k_stride, v_stride, q_stride, q_out_stride, tokens}))
+        return efail(e, SMELT_HIP_ERR_INVALID_ARGUMENT, "paged_kv_append: null shape, q without q_out or negative size");
+    if (rope->head_dim != cache->head_dim) return efail(e, SMELT_HIP_ERR_UNSUPPORTED_GEOMETRY, "paged_kv_append: the cache holds heads of another size");
+    const std::string name = std::string("paged_kv_append") + (q ? "_q" : "") + rope_tail(rope) + "_kv" + std::to_string(cache->kv_heads) + "_p" + std::to_string(cache->page_size);
+    const SmeltBinding* b[] = {&k, &v, &positions, &slots, &table, &cache->k, &cache->v, q, q_out};
+    const uint32_t u[] = {(uint32_t)tokens, (uint32_t)k_stride, (uint32_t)v_stride, (uint32_t)cache->pages, float_bits(rope->amplitude),
+                          (uint32_t)q_heads, (uint32_t)q_stride, (uint32_t)q_out_stride};
+    return emit_serving(e, name, b, q ? 9 : 7, u, q ? 8 : 5, 1u << 4, dynamic != 0);
+}
+
+int smelt_emit_paged_attention(smelt_emitter* e, const SmeltPagedCache* cache, SmeltBinding q, SmeltBinding page_table, SmeltBinding kv_lens, SmeltBinding offsets,
+                               SmeltBinding output, const SmeltBinding* prefix_table, const SmeltBinding* prefix_len, int prefix_pages, int heads,
+                               int q_stride, int pages_per_sequence, float scale, int window, int sequences, int tokens, int dynamic) {
+    if (!e) return SMELT_HIP_ERR_INVALID_ARGUMENT;
+    if (!cache || (prefix_table == nullptr) != (prefix_len == nullptr) ||
+        any_negative({cache->head_dim, cache->kv_heads, cache->page_size, cache->pages, prefix_pages, heads, q_stride, pages_per_sequence, window, sequences, tokens}))
+        return efail(e, SMELT_HIP_ERR_INVALID_ARGUMENT, "paged_attention: null cache, half a prefix or negative size");
+    const bool shared = prefix_table != nullptr;
+    const std::string name = std::string("paged_attention") + (shared ? "_shared" : "") + "_d" + std::to_string(cache->head_dim) + "_h" + std::to_string(heads) +
+                             "_kv" + std::to_string(cache->kv_heads) + "_p" + std::to_string(cache->page_size);
+    const SmeltBinding* b[] = {&q, &cache->k, &cache->v, &page_table, &kv_lens, &offsets, &output, prefix_table, prefix_len};
+    std::vector<uint32_t> u = {(uint32_t)tokens, (uint32_t)sequences, (uint32_t)cache->pages, (uint32_t)pages_per_sequence};
+    if (shared) u.push_back((uint32_t)prefix_pages);
+    u.insert(u.end(), {float_bits(scale), (uint32_t)window, (uint32_t)q_stride});
+    return emit_serving(e, name, b, shared ? 9 : 7, u.data(), (int)u.size(), 1u << (shared ? 5 : 4), dynamic != 0);
+}
+
+int smelt_emit_verify_drafts(smelt_emitter* e, SmeltBinding target, const SmeltBinding* draft, SmeltBinding draft_tokens, SmeltBinding offsets, SmeltBinding u_accept,
+                             SmeltBinding u_sample, SmeltBinding temperature, SmeltBinding tokens, SmeltBinding counts, int rows, int sequences, int vocab,
+                             int stride) {
+    if (!e) return SMELT_HIP_ERR_INVALID_ARGUMENT;
+    if (any_negative({rows, sequences, vocab, stride})) return efail(e, SMELT_HIP_ERR_INVALID_ARGUMENT, "verify_drafts: negative size");
+    std::vector<const SmeltBinding*> b = {&target};
+    if (draft) b.push_back(draft);
+    for (const SmeltBinding* x : {&draft_tokens, &offsets, &u_accept, &u_sample, &temperature, &tokens, &counts}) b.push_back(x);
+    const uint32_t u[] = {(uint32_t)rows, (uint32_t)sequences, (uint32_t)vocab, (uint32_t)stride};
+    return emit_serving(e, draft ? "verify_drafts" : "verify_drafts_given", b.data(), (int)b.size(), u, 4, 0, false);
 }
 
 int smelt_hip_resolve_pipeline_name(const char* entry, int default_act, char* symbol, size_t symbol_cap, char* kinds, size_t kinds_cap) {

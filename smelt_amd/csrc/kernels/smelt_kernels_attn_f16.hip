@@ -1,0 +1,7 @@
+// Attention over the paged cache, f16 (smelt_kernels_attn_f16.hsaco).
+// Built with:  hipcc --offload-arch=gfx950 --genco -O3 -Xclang -target-feature -Xclang -packed-fp32-ops
+#include "paged_attention.hpp"
+
+SMELT_ATTENTION_KERNELS(f16, smelt::F16, 64, 2)
+SMELT_ATTENTION_KERNELS(f16, smelt::F16, 128, 2)
+SMELT_ATTENTION_KERNELS(f16, smelt::F16, 256, 1)

@@ -4,6 +4,7 @@
 // (SmeltKernelCatalog.swift).  The HIP kernels take the shape as arguments, so every name of
 // an in-scope family maps onto a handful of symbols plus appended shape values.
 #include "pipeline_table.hpp"
+#include "serving.hpp"
 
 #include <cstring>
 
@@ -961,8 +962,7 @@ ResolveStatus resolve_pipeline_entry(const std::string& entry_in, ActDType defau
     }
     if (entry == "argmax_key_reduce") { out->family = kFamArgmaxReduce; out->symbol = "smelt_argmax_key_reduce"; out->kinds = "PPU"; return kResolveOk; }
 
-    *why = "no HIP kernel named '" + entry + "'";
-    return kResolveUnknown;
+    return resolve_serving(entry, t.c_str(), out, why);
 }
 
 }  // namespace

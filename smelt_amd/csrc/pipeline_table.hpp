@@ -90,6 +90,14 @@ enum FamilyId {
     kFamNormScaleAffineQmmGateUp,// rs X nw gW gS gB uW uS uB Y batch | rows cols group batch_tile
     kFamAffineDualAdd,           // W1 S1 B1 W2 S2 B2 x y1 y2 res1 res2 | rows cols group          (grid.y = token)
     kFamAffineDualBatched,       // W1 S1 B1 W2 S2 B2 X Y1 Y2 batch | rows cols group batch_tile
+    // serving operators (planned and checked in serving.cpp; the shape in the pipeline's name follows the record's values)
+    kFamRope,                    // x y positions table tokens heads x_stride y_stride amplitude | dim rot interleaved
+    kFamPagedAppend,             // k v positions slots table kcache vcache tokens k_stride v_stride pages amplitude | dim rot interleaved kv_heads page
+    kFamPagedAppendQ,            // ... vcache q q_out tokens k_stride v_stride pages amplitude q_heads q_stride q_out_stride | dim rot interleaved kv_heads page
+    kFamPagedAttention,          // q kcache vcache page_table kv_lens offsets out tokens sequences pages pages_per_seq scale window q_stride | dim heads kv_heads page
+    kFamPagedAttentionShared,    // ... out prefix_table prefix_len tokens sequences pages pages_per_seq prefix_pages scale window q_stride | dim heads kv_heads page
+    kFamVerifyDrafts,            // target draft draft_tokens offsets u_accept u_sample temperature tokens counts rows sequences vocab stride
+    kFamVerifyDraftsGiven,       // target draft_tokens offsets u_accept u_sample temperature tokens counts rows sequences vocab stride
     kFamCount
 };
 
@@ -118,6 +126,7 @@ struct ResolvedPipeline {
     // "smelt_affine_qms_r<R>_x<X>_" + qms_tail for R row tiles per wave and 4 X staged token rows.
     std::string qms_tail;
     uint32_t qms_nmat = 1;
+    std::vector<std::string> serving_symbols;   // kernels of a serving operator; its plan picks by index
 };
 
 constexpr uint32_t kSkinnyVariant = 32;

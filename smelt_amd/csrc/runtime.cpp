@@ -16,6 +16,7 @@
 #include "../../include/smelt_hip.h"
 #include "pipeline_table.hpp"
 #include "runtime_internal.hpp"
+#include "serving.hpp"
 
 using namespace smelt_host;
 
@@ -36,6 +37,7 @@ struct SlotBuffer {
     void* ptr = nullptr;
     size_t bytes = 0;
     bool read_only = false;
+    bool external = false;      // the caller's memory (smelt_hip_buffer_bind): not freed here, no slack behind it
 };
 
 struct Pipeline {
@@ -53,6 +55,7 @@ struct Pipeline {
     hipFunction_t fn_tqs[2] = {};                                 // streaming ternary qmm, eight / sixteen staged token rows
     hipFunction_t fn_norm_rows = nullptr;                         // norm-scale qmm: the normalised rows, written once
     hipFunction_t fn_logits_keys = nullptr;                       // lm_head over several tokens: partial argmax keys from stored logits
+    std::vector<hipFunction_t> fn_serving;                        // serving operators: the kernels their plans pick from
     ResolvedPipeline res;
 };
 
@@ -983,6 +986,67 @@ const Pipeline* pipeline_for(smelt_hip_context* ctx, uint32_t index) {
     return nullptr;
 }
 
+// Serving operators: the geometry follows from the record's values (serving.cpp), the record's own grid and threadgroup are nominal.
+// Returns the number of kernels launched.
+int encode_serving(smelt_hip_context* ctx, const Pipeline& p, const Launch& L, const SplitKWorkspace& ws) {
+    ServingDevice dev;
+    dev.compute_units = (uint32_t)std::max(1, ctx->props.multiProcessorCount);
+    dev.lds_limit = ctx->lds_limit;
+    dev.workspace = ws.partial;
+    dev.workspace_bytes = ws.partial_bytes;
+    ServingPlan plan;
+    uint32_t value[kMaxLaunchArgs] = {};
+    for (size_t i = 0; i < L.args.size(); ++i) {
+        if (L.args[i].kind == 'P') plan.operand[i].ptr = L.args[i].ptr;
+        else value[i] = L.args[i].value;
+    }
+    std::string why;
+    if (int e = plan_serving(p.res, value, dev, &plan, &why)) return fail(ctx, e, "pipeline '" + p.entry + "': " + why);
+    if (plan.steps == 0) return 0;
+    for (int i = 0; i < plan.operands; ++i) {
+        const ServingOperand& o = plan.operand[i];
+        const Arg& a = L.args[(size_t)i];
+        if (o.need > a.avail)
+            return fail(ctx, SMELT_HIP_ERR_OUT_OF_RANGE,
+                        "pipeline '" + p.entry + "': argument " + std::to_string(i) + " needs " + std::to_string(o.need) + " bytes, slot has " +
+                            std::to_string(a.avail) + " from its offset");
+        if (o.need && ((uintptr_t)a.ptr) % o.align != 0)
+            return fail(ctx, SMELT_HIP_ERR_UNSUPPORTED_GEOMETRY,
+                        "pipeline '" + p.entry + "': argument " + std::to_string(i) + " must be " + std::to_string(o.align) + "-byte aligned");
+        if (o.written && !a.writable)
+            return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT,
+                        "pipeline '" + p.entry + "': output argument " + std::to_string(i) + " is bound to the read-only weights slot");
+    }
+    for (int i = 0; i < plan.steps; ++i) {
+        const ServingStep& s = plan.step[i];
+        if (s.lds > ctx->lds_limit)
+            return fail(ctx, SMELT_HIP_ERR_UNSUPPORTED_GEOMETRY, "pipeline '" + p.entry + "': needs " + std::to_string(s.lds) + " bytes of LDS, device allows " + std::to_string(ctx->lds_limit));
+        if ((size_t)s.kernel >= p.fn_serving.size() || !p.fn_serving[(size_t)s.kernel])
+            return fail(ctx, SMELT_HIP_ERR_UNKNOWN_PIPELINE, "pipeline '" + p.entry + "': the loaded code objects miss one of its kernels");
+    }
+    // the stream belongs to the context's device, whatever the calling thread has current
+    int current = ctx->device;
+    HIP_TRY(ctx, hipGetDevice(&current));
+    if (current != ctx->device) HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipError_t err = hipSuccess;
+    if (!ctx->batch_open) {
+        err = hipEventRecord(ctx->ev_start, ctx->stream);
+        ctx->batch_open = err == hipSuccess;
+        ctx->timing_valid = false;
+    }
+    int launched = 0;
+    for (int i = 0; i < plan.steps && err == hipSuccess; ++i) {
+        ServingStep& s = plan.step[i];
+        size_t bytes = s.arg_bytes;
+        void* config[] = {HIP_LAUNCH_PARAM_BUFFER_POINTER, s.args, HIP_LAUNCH_PARAM_BUFFER_SIZE, &bytes, HIP_LAUNCH_PARAM_END};
+        err = hipModuleLaunchKernel(p.fn_serving[(size_t)s.kernel], s.grid[0], s.grid[1], s.grid[2], s.threads, 1, 1, (unsigned)s.lds, ctx->stream, nullptr, config);
+        launched += err == hipSuccess;
+    }
+    if (current != ctx->device) (void)hipSetDevice(current);
+    if (err != hipSuccess) return hip_fail(ctx, err, "launch of a serving kernel");
+    return launched;
+}
+
 // Returns 1 launched, 0 skipped, <0 error.
 int encode_record(smelt_hip_context* ctx, const SmeltDispatchRecord* rec, int cur, int alt, const Dyn& d,
                   const SplitKWorkspace* ws_override = nullptr) {
@@ -1011,6 +1075,9 @@ int encode_record(smelt_hip_context* ctx, const SmeltDispatchRecord* rec, int cu
         size_t off = 0;
         if (int e = resolve_offset(ctx, b, d, &off)) return e;
         const SlotBuffer& sb = ctx->slots[(size_t)slot];
+        // (the other kernels load whole vectors behind a ragged tail, which only the library's own allocations have room for)
+        if (sb.external && !is_serving(p->res.family))
+            return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT, "pipeline '" + p->entry + "' does not take slot " + std::to_string(slot) + ", which is bound to the caller's memory: only the serving operators do");
         if (off > sb.bytes)
             return fail(ctx, SMELT_HIP_ERR_OUT_OF_RANGE, slot == ctx->weights_slot
                             ? "weight offset " + std::to_string(off) + " is outside the mapped weight segments"
@@ -1045,6 +1112,7 @@ int encode_record(smelt_hip_context* ctx, const SmeltDispatchRecord* rec, int cu
     for (size_t i = 0; i < L.args.size(); ++i)
         if (L.args[i].kind == 0)
             return fail(ctx, SMELT_HIP_ERR_BINDING_MISMATCH, "pipeline '" + p->entry + "': argument " + std::to_string(i) + " is not bound by the record");
+    if (is_serving(p->res.family)) return encode_serving(ctx, *p, L, ws);
 
     uint32_t gw = rec->grid_w, gh = rec->grid_h, gd = rec->grid_d;
     if (d.prefill) {
@@ -1500,7 +1568,7 @@ void smelt_hip_context_destroy(smelt_hip_context* ctx) {
     (void)hipSetDevice(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
     for (SlotBuffer& s : ctx->slots)
-        if (s.ptr) (void)hipFree(s.ptr);
+        if (s.ptr && !s.external) (void)hipFree(s.ptr);
     if (ctx->ws_partial) (void)hipFree(ctx->ws_partial);
     if (ctx->ws_counters) (void)hipFree(ctx->ws_counters);
     for (hipModule_t m : ctx->modules) (void)hipModuleUnload(m);
@@ -1607,6 +1675,11 @@ int smelt_hip_pipeline_create(smelt_hip_context* ctx, const char* entry, int all
                 return fail(ctx, SMELT_HIP_ERR_UNKNOWN_PIPELINE, "code object has no kernel '" + p.res.symbol + "' for pipeline '" + p.entry + "': " + hipGetErrorString(e));
         } else {
             p.ready = true;
+            for (const std::string& symbol : p.res.serving_symbols) {
+                hipFunction_t fn = nullptr;
+                (void)find(&fn, symbol);
+                p.fn_serving.push_back(fn);
+            }
             if (!p.res.symbol_single.empty() && find(&p.fn_single, p.res.symbol_single) != hipSuccess) p.fn_single = nullptr;
             if (!p.res.mm1_prefix.empty())
                 for (uint32_t nl = 1; nl <= kMm1MaxSegments; ++nl)
@@ -1659,24 +1732,29 @@ int smelt_hip_pipeline_is_ready(const smelt_hip_context* ctx, uint32_t index) {
     return ctx->pipelines[index].ready ? 1 : 0;
 }
 
+// waits for the stream and gives up what the slot names
+static int clear_slot(smelt_hip_context* ctx, SlotBuffer& s) {
+    if (!s.ptr) return SMELT_HIP_OK;
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+    if (!s.external) HIP_TRY(ctx, hipFree(s.ptr));
+    s = SlotBuffer();
+    return SMELT_HIP_OK;
+}
+
 static int alloc_slot(smelt_hip_context* ctx, int slot, size_t bytes, bool read_only) {
     if (!ctx || slot < 0 || slot >= kMaxSlots) return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT, "slot index out of range");
     if (bytes == 0) return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT, "zero-length buffer");
     if ((size_t)slot >= ctx->slots.size()) ctx->slots.resize((size_t)slot + 1);
     SlotBuffer& s = ctx->slots[(size_t)slot];
     HIP_TRY(ctx, hipSetDevice(ctx->device));
-    if (s.ptr && s.bytes == bytes) {
+    if (s.ptr && !s.external && s.bytes == bytes) {
         // same size: the slot keeps its memory, so that a captured graph that binds it keeps writing to live memory
         HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
         HIP_TRY(ctx, hipMemset(s.ptr, 0, bytes + 256));
         s.read_only = read_only;
         return SMELT_HIP_OK;
     }
-    if (s.ptr) {
-        HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
-        HIP_TRY(ctx, hipFree(s.ptr));
-        s = SlotBuffer();
-    }
+    if (int e = clear_slot(ctx, s)) return e;
     // 256 bytes of slack keep whole-vector loads of a ragged tail inside the allocation
     HIP_TRY(ctx, hipMalloc(&s.ptr, bytes + 256));
     HIP_TRY(ctx, hipMemset(s.ptr, 0, bytes + 256));
@@ -1687,6 +1765,48 @@ static int alloc_slot(smelt_hip_context* ctx, int slot, size_t bytes, bool read_
 
 int smelt_hip_buffer_alloc(smelt_hip_context* ctx, int slot, size_t bytes) {
     return alloc_slot(ctx, slot, bytes, false);
+}
+
+int smelt_hip_buffer_bind(smelt_hip_context* ctx, int slot, void* device_ptr, size_t bytes) {
+    if (!ctx || slot < 0 || slot >= kMaxSlots) return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT, "slot index out of range");
+    if (!device_ptr || bytes == 0) return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT, "null or empty memory");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipPointerAttribute_t attr;
+    memset(&attr, 0, sizeof(attr));
+    const hipError_t known = hipPointerGetAttributes(&attr, device_ptr);
+    if (known != hipSuccess) (void)hipGetLastError();
+    if (known != hipSuccess || attr.type != hipMemoryTypeDevice || attr.device != ctx->device)
+        return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT, "the memory to bind is not on the context's device");
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (hipMemGetAddressRange(&base, &size, device_ptr) == hipSuccess) {
+        const size_t in = (size_t)((char*)device_ptr - (char*)base);
+        if (in > size || bytes > size - in) return fail(ctx, SMELT_HIP_ERR_OUT_OF_RANGE, "the memory to bind ends behind its allocation");
+    } else {
+        (void)hipGetLastError();   // memory mapped by other means has no single range to compare with
+    }
+    if ((size_t)slot >= ctx->slots.size()) ctx->slots.resize((size_t)slot + 1);
+    SlotBuffer& s = ctx->slots[(size_t)slot];
+    if (int e = clear_slot(ctx, s)) return e;
+    if (slot == ctx->weights_slot) ctx->weights_slot = -1;
+    s.ptr = device_ptr;
+    s.bytes = bytes;
+    s.external = true;
+    return SMELT_HIP_OK;
+}
+
+int smelt_hip_buffer_release(smelt_hip_context* ctx, int slot) {
+    if (!ctx || slot < 0 || (size_t)slot >= ctx->slots.size()) return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT, "bad slot");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    if (int e = clear_slot(ctx, ctx->slots[(size_t)slot])) return e;
+    if (slot == ctx->weights_slot) ctx->weights_slot = -1;
+    return SMELT_HIP_OK;
+}
+
+int smelt_hip_context_stream(smelt_hip_context* ctx, void** out_stream) {
+    if (!ctx || !out_stream) return fail(ctx, SMELT_HIP_ERR_INVALID_ARGUMENT, "null argument");
+    *out_stream = ctx->stream;
+    return SMELT_HIP_OK;
 }
 
 int smelt_hip_weights_upload(smelt_hip_context* ctx, int weights_slot, const void* bytes, size_t size) {

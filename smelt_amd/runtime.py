@@ -121,6 +121,9 @@ def load_library() -> C.CDLL:
         "smelt_hip_buffer_write": (i32, [vp, i32, sz, vp, sz]),
         "smelt_hip_buffer_read": (i32, [vp, i32, sz, vp, sz]),
         "smelt_hip_buffer_size": (i32, [vp, i32, C.POINTER(sz)]),
+        "smelt_hip_buffer_bind": (i32, [vp, i32, vp, sz]),
+        "smelt_hip_buffer_release": (i32, [vp, i32]),
+        "smelt_hip_context_stream": (i32, [vp, C.POINTER(vp)]),
         "smelt_hip_weights_upload": (i32, [vp, i32, vp, sz]),
         "smelt_hip_set_cache_seq_capacity": (i32, [vp, u32]),
         "smelt_hip_dispatch_table_count": (i32, [sz, C.POINTER(sz)]),
@@ -215,6 +218,20 @@ class Context:
     # -- buffers -------------------------------------------------------------------------
     def alloc(self, slot: int, nbytes: int) -> None:
         self.check(self.lib.smelt_hip_buffer_alloc(self.h, slot, nbytes))
+
+    def bind(self, slot: int, device_ptr: int, nbytes: int) -> None:
+        """Name `nbytes` of the caller's device memory by `slot` (serving operators only); it must outlive the binding."""
+        self.check(self.lib.smelt_hip_buffer_bind(self.h, slot, device_ptr, nbytes))
+
+    def release(self, slot: int) -> None:
+        """Free what `slot` names, or forget it when it is bound."""
+        self.check(self.lib.smelt_hip_buffer_release(self.h, slot))
+
+    def stream(self) -> int:
+        """The hipStream_t that every record of this context runs on."""
+        v = C.c_void_p()
+        self.check(self.lib.smelt_hip_context_stream(self.h, C.byref(v)))
+        return v.value or 0
 
     def upload_weights(self, slot: int, data: np.ndarray) -> None:
         data = np.ascontiguousarray(data)

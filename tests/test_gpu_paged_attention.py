@@ -1,0 +1,246 @@
+"""Attention over the paged cache against the softmax in 64 bits, at the sizes and masks where it can go wrong."""
+import numpy as np
+import pytest
+
+import fixtures as fx
+import serving_ref as sr
+from smelt_amd import compiler as cc
+from smelt_amd import runtime as rt
+
+pytestmark = pytest.mark.gpu
+B = cc.bind
+ACT = {fx.F16: rt.ACT_F16, fx.BF16: rt.ACT_BF16}
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = rt.Context()
+    yield c
+    c.close()
+
+
+class Case:
+    """Operands in slots 1.. of a batch: new tokens n, own keys L (new ones included), a prefix."""
+
+    def __init__(self, ctx, dtype, n, L, heads, kv_heads, dim, page, prefix=0, window=0, pad=0, gap=0, scale=None, seed=0, poison=True, width=None):
+        self.__dict__.update(locals())
+        rng = fx.rng_for(220, seed + dim + page + sum(L))
+        self.sequences = len(n)
+        self.offsets = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+        self.tokens = int(self.offsets[-1]) + pad
+        used = [-(-l // page) for l in L]
+        front = -(-prefix // page)
+        self.width = width or max(1, max(used))
+        self.pages = sum(used) + front + 2
+        order = rng.permutation(self.pages)
+        self.prefix_pages = order[:front].astype(np.int32)
+        self.table = np.full((self.sequences, self.width), 2 ** 30, np.int32)       # entries behind a sequence's end name no page
+        at = front
+        for s, u in enumerate(used):
+            self.table[s, :u] = order[at:at + u]
+            at += u
+        self.qb, q = sr.values(rng, (self.tokens, heads * dim + gap), dtype, 2.0)
+        kb, k = sr.values(rng, (self.pages, kv_heads, page, dim), dtype)
+        vb, v = sr.values(rng, (self.pages, kv_heads, page, dim), dtype)
+        self.kb, self.vb = kb, vb
+        if poison:       # infinities and NaN wherever no sequence has written
+            owned = np.zeros((self.pages, page), bool)
+            for j in range(prefix):
+                owned[self.prefix_pages[j // page], j % page] = True
+            for s, l in enumerate(L):
+                for j in range(l):
+                    owned[self.table[s, j // page], j % page] = True
+            bad = np.array([0x7E00, 0x7C00, 0xFC00] if dtype == fx.F16 else [0x7FC0, 0x7F80, 0xFF80], np.uint16)
+            for x in (kb, vb):
+                free = ~owned[:, None, :, None] & np.ones(x.shape, bool)
+                x[free] = bad[rng.integers(0, 3, int(free.sum()))]
+        self.q = q[:, :heads * dim].reshape(self.tokens, heads, dim)
+        self.lens = np.array(L, np.int32)
+        self.scale = 1.0 / np.sqrt(dim) if scale is None else scale
+        self.out0 = rng.integers(0, 30000, (self.tokens, heads * dim)).astype(np.uint16)
+
+    def load(self):
+        c = self.ctx
+        c.put(1, self.qb); c.put(2, sr.keys_to_pages(self.kb, self.page)); c.put(3, self.vb); c.put(4, self.table); c.put(5, self.lens); c.put(6, self.offsets)
+        c.put(7, self.out0)
+        if self.prefix:
+            c.put(8, self.prefix_pages); c.put(9, np.array([self.prefix], np.int32))
+        em = cc.Emitter(act_dtype=ACT[self.dtype])
+        shared = dict(prefix_table=B(8), prefix_len=B(9), prefix_pages=len(self.prefix_pages)) if self.prefix else {}
+        em.paged_attention(B(1), B(2), B(3), B(4), B(5), B(6), B(7), self.tokens, self.sequences, self.heads, self.kv_heads, self.dim, self.page, self.pages, self.width,
+                           self.scale, window=self.window, q_stride=self.heads * self.dim + self.gap, **shared)
+        return em.table_for(c)
+
+    def result(self):
+        return self.ctx.read(7, np.uint16, self.out0.size).reshape(self.out0.shape)
+
+    def want(self):
+        k, v = sr.wide(self.kb, self.dtype), sr.wide(self.vb, self.dtype)
+        return sr.attention(self.q, k, v, self.pages, self.table, self.lens, self.offsets, float(np.float32(self.scale)), self.window, self.prefix_pages, self.prefix)
+
+    def check(self, got):
+        y, reach, sharp, count = self.want()
+        live = int(self.offsets[-1])
+        assert np.array_equal(got[live:], self.out0[live:])                        # rows behind the last sequence
+        tol = sr.attention_tolerance(y, reach, sharp, count, self.dim, self.dtype)[:live]
+        g = sr.wide(got[:live], self.dtype).reshape(y[:live].shape)
+        assert np.array_equal(np.isnan(g), np.isnan(y[:live])) and np.isfinite(g).all()
+        off = np.abs(g - y[:live])
+        assert np.all(off <= tol), f"{(off / tol).max():.2f} of the tolerance at {np.unravel_index((off / tol).argmax(), off.shape)}"
+
+    def run(self):
+        table = self.load()
+        self.ctx.interpret_decode(table)
+        self.ctx.wait()
+        self.check(self.result())
+        return self
+
+
+TYPES = pytest.mark.parametrize("dtype", [fx.F16, fx.BF16], ids=["f16", "bf16"])
+
+
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_one_token_a_sequence(ctx, dtype, dim, page):
+    Case(ctx, dtype, [1] * 7, [1, 2, 31, 32, 33, 300, 65], 6, 2, dim, page, pad=2, gap=8).run()
+
+
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("prefix", [1, 40, 200])
+def test_shared_prefix(ctx, dtype, dim, page, prefix):
+    Case(ctx, dtype, [1, 0, 4, 1, 7], [1, 50, 4, 90, 33], 12, 2, dim, page, prefix=prefix, pad=1).run()
+
+
+@TYPES
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (5, 1), (8, 8), (24, 4), (33, 1), (64, 2)])
+def test_head_layouts(ctx, dtype, heads, kv_heads):
+    Case(ctx, dtype, [1, 3, 2], [70, 3, 129], heads, kv_heads, 64, 32, prefix=45).run()
+
+
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page,prefix", [(16, 0), (64, 0), (16, 37), (64, 100), (256, 0)])
+def test_prompts(ctx, dtype, dim, page, prefix):
+    """Many rows a sequence, behind earlier keys and from nothing."""
+    Case(ctx, dtype, [75, 1, 40], [75, 20, 161], 4, 2, dim, page, prefix=prefix).run()
+
+
+@TYPES
+@pytest.mark.parametrize("window", [1, 5, 32, 100])
+@pytest.mark.parametrize("prefix", [0, 90])
+def test_windows(ctx, dtype, window, prefix):
+    """Rows that see no prefix, part of it, one key."""
+    Case(ctx, dtype, [1, 9, 1, 50], [1, 30, 200, 64], 4, 2, 64, 16, prefix=prefix, window=window).run()
+
+
+@TYPES
+@pytest.mark.parametrize("prefix", [0, 20])
+def test_rows_that_see_nothing(ctx, dtype, prefix):
+    """No keys at all; fewer keys than new rows (the first rows stand before key 0)."""
+    c = Case(ctx, dtype, [2, 5, 1], [0, 2, 3], 4, 2, 64, 16, prefix=prefix).run()
+    if not prefix:
+        assert not c.result()[:2].any() and not c.result()[2:5].any()
+
+
+@TYPES
+def test_long_and_short_together(ctx, dtype):
+    """One sequence holds most of the keys: its segments are cut over many workgroups and joined."""
+    Case(ctx, dtype, [1, 2, 1, 1], [17, 9000, 1, 64], 4, 2, 128, 64, prefix=0, seed=3).run()
+    Case(ctx, dtype, [1, 2], [17, 90], 2, 1, 256, 64, prefix=6000, seed=4).run()
+
+
+@TYPES
+def test_many_sequences(ctx, dtype):
+    """More sequences than a workgroup has threads, some without rows."""
+    rng = fx.rng_for(221, 0)
+    n = rng.integers(0, 3, 300)
+    L = np.maximum(rng.integers(0, 60, 300), n)
+    Case(ctx, dtype, n.tolist(), L.tolist(), 2, 1, 64, 16, prefix=33, pad=3).run()
+
+
+@TYPES
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+def test_scales(ctx, dtype, scale):
+    Case(ctx, dtype, [1, 4], [40, 100], 4, 2, 64, 32, scale=scale, prefix=17).run()
+
+
+def test_odd_row_strides_of_q(ctx):
+    Case(ctx, fx.F16, [1, 3], [40, 70], 3, 3, 64, 32, gap=3).run()
+
+
+@TYPES
+def test_pages_outside_the_pool_are_not_seen(ctx, dtype):
+    """A table entry that names no page of the pool hides its keys: the result is the one without them."""
+    for page, hidden in ((16, -1), (64, 2 ** 30)):
+        c = Case(ctx, dtype, [1, 2], [200, 150], 4, 2, 64, page, prefix=2 * page + 5)
+        c.table[0, 1] = hidden
+        c.prefix_pages[1] = hidden
+        c.run()
+
+
+def test_lengths_are_cut_to_what_the_tables_hold(ctx):
+    c = Case(ctx, fx.F16, [1, 1], [64, 50], 2, 1, 64, 16, prefix=32)
+    want = c.load()
+    c.ctx.interpret_decode(want); c.ctx.wait()
+    first = c.result().copy()
+    c.ctx.put(5, np.array([1 << 30, 50], np.int32)); c.ctx.put(9, np.array([1 << 30], np.int32))
+    c.ctx.interpret_decode(want); c.ctx.wait()
+    assert np.array_equal(c.result()[0], first[0])
+    c.ctx.put(5, np.array([-5, 50], np.int32)); c.ctx.put(9, np.array([-1], np.int32))
+    c.ctx.interpret_decode(want); c.ctx.wait()
+    assert not c.result()[0].any() and c.result()[1].any()
+
+
+def test_infinities_and_nans_that_are_seen(ctx):
+    """A NaN score makes its rows NaN and no others; a score of -inf is a key that is not seen."""
+    c = Case(ctx, fx.BF16, [1, 1, 1], [40, 60, 33], 2, 1, 64, 32)
+    at = lambda s, j: (c.table[s, j // 32], 0, j % 32)   # noqa: E731
+    c.kb[at(0, 5)] = 0x7FC0
+    c.kb[at(2, 7)] = 0
+    c.kb[at(2, 7)][0] = 0xFF80                             # q0 * -inf
+    sign = c.qb[2, :].reshape(2, 64)[:, 0]
+    assert np.all(sr.wide(sign, fx.BF16) != 0)
+    c.qb[2, 0::64] &= 0x7FFF                               # q0 positive: the score is -inf
+    c.q = sr.wide(c.qb, fx.BF16).reshape(3, 2, 64)
+    t = c.load()
+    c.ctx.interpret_decode(t); c.ctx.wait()
+    g = sr.wide(c.result(), fx.BF16)
+    assert np.isnan(g[0]).all() and np.isfinite(g[1:]).all()
+    y, reach, sharp, count = c.want()
+    tol = sr.attention_tolerance(y, reach, np.where(np.isfinite(sharp), sharp, 20.0), count, 64, fx.BF16)
+    assert np.all(np.abs(g[1:].reshape(2, 2, 64) - y[1:]) <= tol[1:])
+
+
+def test_the_same_inputs_give_the_same_bits(ctx):
+    c = Case(ctx, fx.BF16, [1, 5, 3, 1], [700, 2000, 64, 1], 8, 2, 128, 64, prefix=900)
+    t = c.load()
+    c.ctx.interpret_decode(t); c.ctx.wait()
+    first = c.result().copy()
+    for _ in range(3):
+        c.ctx.interpret_decode(t)
+    c.ctx.wait()
+    assert np.array_equal(first, c.result())
+
+
+def test_attention_is_refused_where_a_slot_is_short(ctx):
+    c = Case(ctx, fx.F16, [1, 2], [40, 70], 4, 2, 64, 16, prefix=20)
+    c.load()
+
+    def go(**kw):
+        a = dict(q=B(1), k_cache=B(2), v_cache=B(3), page_table=B(4), kv_lens=B(5), offsets=B(6), out=B(7), tokens=3, sequences=2, heads=4, kv_heads=2, head_dim=64, page_size=16,
+                 pages=c.pages, pages_per_sequence=c.width, scale=0.1, prefix_table=B(8), prefix_len=B(9), prefix_pages=2)
+        em = cc.Emitter()
+        em.paged_attention(**{**a, **kw})
+        return ctx.interpret_decode(em.table_for(ctx))
+
+    assert go() >= 1 and go(tokens=0) == 0 and go(sequences=0) == 0
+    for kw in (dict(tokens=4), dict(pages=c.pages + 1), dict(pages_per_sequence=c.width + 1), dict(sequences=3), dict(prefix_pages=3), dict(out=B(7, 16)), dict(kv_lens=B(5, 4)),
+               dict(q_stride=512), dict(k_cache=B(2, 16))):
+        with pytest.raises(rt.SmeltHipError, match="needs"):
+            go(**kw)
+    with pytest.raises(rt.SmeltHipError, match="aligned"):
+        go(tokens=1, sequences=1, out=B(7, 2))
+    ctx.wait()

@@ -1,0 +1,223 @@
+"""Serving operators without a GPU: pipeline names, what the emitters refuse, frequency tables, the attention's work partition."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from smelt_amd import compiler as cc
+from smelt_amd import runtime as rt
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+B = cc.bind
+
+
+@pytest.mark.parametrize("name,symbol", [
+    ("rope_half_d256_r64", "smelt_rope_vec_f16"), ("rope_interleaved_d100_r20@bf16", "smelt_rope_vec_bf16"),
+    ("paged_kv_append_half_d128_r0_kv8_p16", "smelt_paged_append_vec_f16"),
+    ("paged_kv_append_q_interleaved_d64_r64_kv1_p256", "smelt_paged_append_vec_f16"),
+    ("paged_attention_d256_h24_kv4_p64", "smelt_attention_stream_d256_f16"),
+    ("paged_attention_shared_d64_h6_kv2_p16@bf16", "smelt_attention_stream_d64_p16_bf16"),
+    ("verify_drafts", "smelt_verify_stats_f16"), ("verify_drafts_given@bf16", "smelt_verify_stats_bf16")])
+def test_names_resolve(name, symbol):
+    rc, sym, kinds = cc.resolve_pipeline_name(name)
+    assert rc == 0 and sym == symbol and set(kinds) <= set("PUF")
+
+
+@pytest.mark.parametrize("name,code", [
+    ("rope_half_d256_r63", -3), ("rope_half_d64_r128", -3), ("rope_half_d64_r0", -3), ("rope_half_d2000_r64", -3), ("rope_d64_r64", -4),
+    ("rope_half_d64", -4), ("rope_half_d64_r64_x", -4), ("paged_kv_append_half_d96_r64_kv4_p64", -3),
+    ("paged_kv_append_half_d64_r64_kv4_p24", -3), ("paged_kv_append_half_d64_r64_kv0_p16", -3), ("paged_kv_append_half_d64_r64_kv4", -4),
+    ("paged_attention_d80_h8_kv8_p16", -3), ("paged_attention_d64_h8_kv3_p16", -3), ("paged_attention_d64_h0_kv1_p16", -3),
+    ("paged_attention_d64_h8_kv2_p48", -3), ("paged_attention_d64_h8_kv2_p99999999999", -4), ("paged_attention", -4), ("verify_drafts_x", -4)])
+def test_names_refused(name, code):
+    assert cc.resolve_pipeline_name(name)[0] == code
+
+
+def refused(call, *words):
+    with pytest.raises(cc.EmitError) as e:
+        call()
+    for w in words:
+        assert w in e.value.message, e.value.message
+
+
+def test_rope_refusals():
+    em = cc.Emitter()
+    ok = dict(tokens=4, heads=8, head_dim=64, rotary_dim=64)
+    em.rope(B(1), B(2), B(3), B(4), **ok)
+    em.rope(B(1), B(1), B(3), B(4), **ok)                                         # in place
+    refused(lambda: em.rope(B(1), B(2), B(3), B(4), **{**ok, "heads": 0}), "heads")
+    refused(lambda: em.rope(B(1), B(2), B(3), B(4), **{**ok, "tokens": -1}), "negative")
+    refused(lambda: em.rope(B(1), B(2), B(3), B(4), x_stride=500, **ok), "stride")
+    refused(lambda: em.rope(B(1), B(2), B(3), B(4), y_stride=511, **ok), "stride")
+    refused(lambda: em.rope(B(1), B(1), B(3), B(4), x_stride=1024, **ok), "overlaps")
+    refused(lambda: em.rope(B(1), B(1, 64), B(3), B(4), **ok), "overlaps")
+    refused(lambda: em.rope(B(1), B(3), B(3), B(4), **ok), "overlaps")
+    refused(lambda: em.rope(B(1), B(2), B(3), B(4), **{**ok, "rotary_dim": 65}), "rotated")
+    refused(lambda: em.rope(B(1), B(2), B(3), B(4), tokens=4, heads=1024, head_dim=1024, rotary_dim=64), "pieces")
+    assert len(em.records()) == 2
+
+
+def test_append_refusals():
+    em = cc.Emitter()
+
+    def go(**kw):
+        a = dict(k=B(1), v=B(2), positions=B(3), slots=B(4), table=B(5), k_cache=B(6), v_cache=B(7), tokens=3, kv_heads=2, head_dim=64, rotary_dim=32, page_size=16, pages=10)
+        em.paged_kv_append(**{**a, **kw})
+
+    go()
+    go(q=B(8), q_out=B(8), q_heads=4)
+    go(rotary_dim=0)
+    refused(lambda: go(q=B(8)), "q without q_out")
+    refused(lambda: go(q=B(8), q_out=B(9), q_heads=0), "heads")
+    refused(lambda: go(q=B(8), q_out=B(1), q_heads=4), "overlaps")
+    refused(lambda: go(pages=0), "pool")
+    refused(lambda: go(pages=2 ** 28), "pool")
+    refused(lambda: go(kv_stride=100), "stride")
+    refused(lambda: go(v_stride=64), "stride")
+    refused(lambda: go(v_cache=B(6)), "overlaps")
+    refused(lambda: go(k_cache=B(1)), "overlaps")
+    refused(lambda: go(head_dim=96), "64, 128 or 256")
+    refused(lambda: go(page_size=8), "pages hold")
+
+
+def test_attention_refusals():
+    em = cc.Emitter()
+
+    def go(**kw):
+        a = dict(q=B(1), k_cache=B(2), v_cache=B(3), page_table=B(4), kv_lens=B(5), offsets=B(6), out=B(7), tokens=4, sequences=2, heads=8, kv_heads=2, head_dim=128,
+                 page_size=64, pages=100, pages_per_sequence=20, scale=0.1)
+        em.paged_attention(**{**a, **kw})
+
+    go()
+    go(prefix_table=B(8), prefix_len=B(9), prefix_pages=3)
+    go(prefix_table=B(8), prefix_len=B(9), prefix_pages=0)
+    refused(lambda: go(prefix_table=B(8)), "half a prefix")
+    refused(lambda: go(out=B(1)), "overlaps")
+    refused(lambda: go(out=B(3)), "overlaps")
+    refused(lambda: go(scale=float("inf")), "finite")
+    refused(lambda: go(scale=float("nan")), "finite")
+    refused(lambda: go(q_stride=1000), "stride")
+    refused(lambda: go(pages_per_sequence=0), "page")
+    refused(lambda: go(pages=0), "pool")
+    refused(lambda: go(heads=7), "multiple")
+    refused(lambda: go(window=-1), "negative")
+    refused(lambda: go(pages_per_sequence=2 ** 25), "positions")
+
+
+def test_verify_refusals():
+    em = cc.Emitter()
+
+    def go(**kw):
+        a = dict(target=B(1), draft_tokens=B(2), offsets=B(3), u_accept=B(4), u_sample=B(5), temperature=B(6), tokens=B(7), counts=B(8), rows=5, sequences=2, vocab=100)
+        em.verify_drafts(**{**a, **kw})
+
+    go()
+    go(draft=B(9))
+    go(draft=B(1))                       # a draft model that is the target
+    refused(lambda: go(stride=99), "stride")
+    refused(lambda: go(vocab=0), "vocabulary")
+    refused(lambda: go(rows=70000), "65535")
+    refused(lambda: go(tokens=B(2)), "overlaps")
+    refused(lambda: go(counts=B(7)), "overlaps")
+    refused(lambda: go(rows=65535, vocab=10 ** 7), "workspace")
+
+
+def test_table_for_looks_pipelines_up_by_type():
+    em = cc.Emitter(act_dtype=rt.ACT_BF16)
+    em.rope(B(1), B(2), B(3), B(4), tokens=4, heads=8, head_dim=64, rotary_dim=64)
+    em16 = cc.Emitter()
+    em16.rope(B(1), B(2), B(3), B(4), tokens=4, heads=8, head_dim=64, rotary_dim=64, dynamic=True)
+
+    class Stub:
+        names = ["something else"]
+
+        def pipeline(self, name):
+            if name not in self.names:
+                self.names.append(name)
+            return self.names.index(name)
+
+    ctx = Stub()
+    assert [r.pipeline for r in em.table_for(ctx)] == [1] and [r.pipeline for r in em16.table_for(ctx)] == [2]
+    assert ctx.names[1:] == ["rope_half_d64_r64@bf16", "rope_half_d64_r64@f16"]
+    assert em16.records()[0].constants[0].kind == rt.CONST_SEQ_LEN
+
+
+@pytest.mark.parametrize("rot", [2, 64, 96, 128])
+def test_rope_tables(rot):
+    i = np.arange(rot // 2)
+    f = 10000.0 ** (-2.0 * i / rot)
+    near = dict(rtol=1e-14, atol=0)
+    t, a = cc.rope_table(rot)
+    assert a == 1.0 and np.allclose(t[:rot // 2], f, **near)
+    assert np.allclose(cc.rope_table(rot, kind=cc.ROPE_LINEAR, factor=8.0)[0][:rot // 2], f / 8, **near)
+    if rot > 2:
+        t = cc.rope_table(rot, kind=cc.ROPE_BASE, factor=8.0)[0]
+        assert t[0] == 1.0 and np.isclose(t[-1], f[-1] / 8, rtol=1e-12)
+    t, a = cc.rope_table(rot, base=500000.0, kind=cc.ROPE_BANDS, factor=8.0, positions=8192.0, low=1.0, high=4.0)
+    g = 500000.0 ** (-2.0 * i / rot)
+    turns = 8192.0 * g / (2 * np.pi)
+    keep = np.clip((turns - 1.0) / 3.0, 0, 1)
+    assert a == 1.0 and np.allclose(t[:rot // 2], keep * g + (1 - keep) * g / 8, rtol=1e-12)
+    t, a = cc.rope_table(rot, kind=cc.ROPE_PARTS, factor=4.0, positions=4096.0, low=1.0, high=32.0)
+    lo, hi = (rot * np.log(4096.0 / (n * 2 * np.pi)) / (2 * np.log(10000.0)) for n in (32.0, 1.0))
+    lo, hi = max(np.floor(lo), 0), min(np.ceil(hi), rot - 1)
+    keep = 1 - np.clip((i - lo) / max(hi - lo, 0.001), 0, 1)
+    assert np.isclose(a, 0.1 * np.log(4.0) + 1, rtol=1e-6) and np.allclose(t[:rot // 2], keep * f + (1 - keep) * f / 4, rtol=1e-12)
+
+
+def test_rope_table_refusals():
+    for kw in (dict(rotary_dim=0), dict(rotary_dim=7), dict(rotary_dim=8, base=0.0), dict(rotary_dim=8, kind=9, factor=2.0), dict(rotary_dim=8, kind=cc.ROPE_LINEAR, factor=0.0),
+               dict(rotary_dim=8, kind=cc.ROPE_BANDS, factor=2.0, low=4.0, high=4.0), dict(rotary_dim=8, kind=cc.ROPE_PARTS, factor=2.0, positions=0.0),
+               dict(rotary_dim=2, kind=cc.ROPE_BASE, factor=2.0), dict(rotary_dim=8, base=float("nan"))):
+        with pytest.raises(ValueError):
+            cc.rope_table(**kw)
+
+
+@pytest.fixture(scope="module")
+def partition(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("partition") / "libpartition.so")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-o", out, os.path.join(HERE, "serving_partition_check.cpp")], check=True)
+    lib = C.CDLL(out)
+    lib.check_owners.restype = C.c_uint64
+    lib.check_owners.argtypes = [C.c_uint64, C.c_uint32]
+    return lib
+
+
+def entries(lib, offsets, lens, tokens, group=1, kv_heads=1, shift=4, width=4, prefix=None, prefix_pages=0, cascade=0):
+    offsets, lens = np.array(offsets, np.int32), np.array(lens, np.int32)
+    out, units = np.zeros((len(lens) + 1, 8), np.int64), C.c_uint64()
+    p = None if prefix is None else C.byref(C.c_int32(prefix))
+    i32p = C.POINTER(C.c_int32)
+    n = lib.check_entries(offsets.ctypes.data_as(i32p), lens.ctypes.data_as(i32p), len(lens), tokens, group, kv_heads, shift, width, p, prefix_pages, cascade,
+                          out.ctypes.data_as(C.POINTER(C.c_int64)), C.byref(units))
+    keys = ("first", "tokens", "row_tiles", "front", "own", "front_tiles", "key_tiles", "sequence")
+    return [dict(zip(keys, r)) for r in out[:n].tolist()], units.value
+
+
+def test_entries_are_cut_to_what_the_tables_hold(partition):
+    # lengths past the table, negative lengths, offsets outside the rows or falling
+    e, units = entries(partition, [0, 3, 3, -5, 900], [1000, 7, -4, 64], tokens=10, group=12, kv_heads=2)
+    assert [x["own"] for x in e] == [64, 7, 0, 64] and [x["tokens"] for x in e] == [3, 0, 0, 10]
+    assert [x["first"] for x in e] == [0, 3, 3, 0] and [x["key_tiles"] for x in e] == [2, 1, 1, 2] and [x["row_tiles"] for x in e] == [2, 0, 0, 4]
+    assert units == 2 * (2 * 2 + 4 * 2)
+    # a prefix longer than its table; the prefix entry covers the rows that belong to a sequence
+    e, units = entries(partition, [0, 1, 2], [5, 0], tokens=4, prefix=1 << 30, prefix_pages=3, cascade=1)
+    assert e[0] == dict(first=0, tokens=2, row_tiles=1, front=48, own=0, front_tiles=2, key_tiles=2, sequence=-1)
+    assert [x["key_tiles"] for x in e[1:]] == [1, 1] and units == 2 + 1 + 1
+    e, _ = entries(partition, [0, 1], [0], tokens=4, prefix=-3, prefix_pages=3, cascade=1)
+    assert e[0]["key_tiles"] == 0 and e[1]["key_tiles"] == 1
+    e, _ = entries(partition, [0, 1], [33], tokens=4, prefix=40, prefix_pages=3)
+    assert (e[0]["front_tiles"], e[0]["key_tiles"]) == (2, 4)
+
+
+def test_every_unit_has_one_workgroup(partition):
+    for units in (1, 2, 3, 4, 5, 63, 64, 1000, 1021, 4096, 100003):
+        for workgroups in (1, 2, 7, 256, 512):
+            assert partition.check_owners(units, workgroups) == 0, (units, workgroups)
+
+
+def test_reciprocal_division_is_exact(partition):
+    for d in (1, 2, 3, 5, 7, 12, 17, 24, 96, 100, 255, 256, 1000, 4095, 4097, 65535):
+        assert partition.check_reciprocal(d, min(2 ** 32 // max(d, 1) - 1, 70000)) == 0, d
