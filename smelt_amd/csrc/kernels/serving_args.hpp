@@ -118,13 +118,21 @@ SMELT_HD uint32_t attention_owner(uint64_t units, uint32_t groups, uint64_t u) {
 }
 
 // ---- verification of drafted tokens ----------------------------------------------------------------------------------
-// Rows are cut into `chunks` runs of `chunk` logits (a multiple of kVerifyStep); the launches leave a record per run.
-constexpr uint32_t kVerifyStep = 2048;     // logits that 256 threads load 16 bytes at a time
+// A row's logits are cut into `runs` runs of `span` (a multiple of kVerifyStep), each the work of one wave; the launches leave a
+// record per run.
+constexpr uint32_t kVerifyStep = 512;      // logits that a wave loads 16 bytes at a time
+constexpr uint32_t kVerifyMaxSpan = 4096;  // four logits a thread of the last launch
 
 struct VerifyStat {
     float top;          // largest logit of the run, -inf when there is none
-    uint32_t where;     // its lowest index
-    double sum;         // sum of exp((logit - top) / temperature)
+    float sum;          // sum of exp((logit - top) / temperature)
+};
+
+// what the second launch leaves of a sequence
+struct VerifyChoice {
+    uint32_t taken;     // accepted drafts
+    uint32_t where;     // greedy: the token to draw (~0: none)
+    float top, draft_top;   // largest logits of the chosen row
 };
 
 struct VerifyArgs {
@@ -137,11 +145,12 @@ struct VerifyArgs {
     const float* temperature = nullptr;
     int32_t* tokens = nullptr;
     int32_t* counts = nullptr;
-    VerifyStat* stats = nullptr;             // [2][rows][chunks]: target, draft
-    double* sums = nullptr;                  // [sequences][3][chunks]: target, draft, leftover of the chosen row
-    int32_t* choice = nullptr;               // [sequences]: accepted drafts
+    VerifyStat* stats = nullptr;             // [2][rows][runs]: target, draft
+    uint32_t* where = nullptr;               // [rows][runs]: lowest index of the target run's largest logit (greedy rows)
+    double* sums = nullptr;                  // [sequences][3][runs]: target, draft, leftover of the chosen row
+    VerifyChoice* choice = nullptr;          // [sequences]
     uint32_t rows = 0, sequences = 0, vocab = 0, stride = 0;
-    uint32_t chunks = 0, chunk = 0, vector = 0;
+    uint32_t runs = 0, span = 0, vector = 0;
 };
 
 SMELT_HD uint32_t reciprocal(uint32_t d) { return d <= 1 ? 0u : (uint32_t)((0x100000000ull + d - 1) / d); }

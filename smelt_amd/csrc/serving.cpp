@@ -317,21 +317,23 @@ int Planner::verify() {
     a.u_accept = P<float>(n + 2); a.u_sample = P<float>(n + 3); a.temperature = P<float>(n + 4);
     a.tokens = P<int32_t>(n + 5); a.counts = P<int32_t>(n + 6);
     a.vector = a.stride % 8 == 0 && aligned16(a.target) && (given || aligned16(a.draft)) ? 1u : 0u;
-    // runs of 2048 logits up to 16384, as long as there are four workgroups a compute unit
-    uint32_t steps = 8;
-    while (steps > 1 && (uint64_t)a.rows * n * ((a.vocab + steps * kVerifyStep - 1) / (steps * kVerifyStep)) < 4ull * dev.compute_units) steps /= 2;
-    a.chunk = steps * kVerifyStep;
-    a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
-    const size_t stats = (size_t)2 * a.rows * a.chunks * sizeof(VerifyStat), sums = (size_t)a.sequences * 3 * a.chunks * 8;
-    if (stats + sums + (size_t)a.sequences * 4 > dev.workspace_bytes)
-        return bad("the runs' records (" + std::to_string(stats + sums) + " bytes) exceed the workspace (" + std::to_string(dev.workspace_bytes) + " bytes)");
+    // runs of 512 logits up to 4096, as long as there are eight waves a compute unit
+    a.span = kVerifyMaxSpan;
+    while (a.span > kVerifyStep && (uint64_t)a.rows * n * ((a.vocab + a.span - 1) / a.span) < 8ull * dev.compute_units) a.span /= 2;
+    a.runs = (a.vocab + a.span - 1) / a.span;
+    const size_t stats = (size_t)2 * a.rows * a.runs * sizeof(VerifyStat), sums = (size_t)a.sequences * 3 * a.runs * 8;
+    const size_t where = (size_t)a.rows * a.runs * 4, all = stats + sums + (size_t)a.sequences * sizeof(VerifyChoice) + where;
+    if (all > dev.workspace_bytes)
+        return bad("the runs' records (" + std::to_string(all) + " bytes) exceed the workspace (" + std::to_string(dev.workspace_bytes) + " bytes)");
     char* ws = static_cast<char*>(dev.workspace);
     a.stats = reinterpret_cast<VerifyStat*>(ws);
     a.sums = reinterpret_cast<double*>(ws + stats);
-    a.choice = reinterpret_cast<int32_t*>(ws + stats + sums);
-    step(0, a, a.chunks, a.rows, (uint32_t)n, 256, 0);
-    step(1, a, a.chunks, a.sequences, 1, 256, 0);
-    if (!given) step(2, a, a.chunks, a.sequences, 1, 256, 0);
+    a.choice = reinterpret_cast<VerifyChoice*>(ws + stats + sums);
+    a.where = reinterpret_cast<uint32_t*>(ws + stats + sums + (size_t)a.sequences * sizeof(VerifyChoice));
+    const uint32_t groups = (a.runs + 3) / 4;
+    step(0, a, groups, a.rows, (uint32_t)n, 256, 0);
+    step(1, a, groups, a.sequences, 1, 256, 0);
+    if (!given) step(2, a, groups, a.sequences, 1, 256, 0);
     step(3, a, a.sequences, 1, 1, 1024, 0);
     return 0;
 }

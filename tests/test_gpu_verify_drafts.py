@@ -94,6 +94,13 @@ def test_all_outcomes_occur(ctx):
     assert np.all(counts == 4)
 
 
+def test_more_runs_than_threads(ctx):
+    """A vocabulary whose runs the last launch walks in several rounds."""
+    for given in (False, True):
+        c = batch(fx.rng_for(242, int(given)), fx.F16, [2, 1], 540001, given=given)
+        check(ctx, c)
+
+
 @TYPES
 def test_more_rows_than_waves(ctx, dtype):
     c = batch(fx.rng_for(232, 0), dtype, [40, 1, 13], 900, near=0.01)
