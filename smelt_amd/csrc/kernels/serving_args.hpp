@@ -40,13 +40,13 @@ struct RopeArgs {
 
 // ---- attention over the paged cache ----------------------------------------------------------------------------------
 // Sequence s has the token rows offsets[s] .. offsets[s + 1] and kv_lens[s] keys of its own, its new tokens' included, on the
-// pages of its row of the page table; keys 0 .. prefix_len of every sequence are the shared prefix.  A launch covers a list
-// of work entries: with `cascade` entry 0 is the prefix against all rows at once and entry s + 1 the sequence's own keys; without it
-// entry s is the sequence's prefix keys and own keys.  An entry is cut into (kv head, tile of kRowTile rows) segments of `key_tiles`
-// tiles of kKeyTile keys, in that order, and the workgroups take equal runs of the resulting units.
-constexpr uint32_t kRowTile = 32;
+// pages of its row of the page table; keys 0 .. prefix_len of every sequence are the shared prefix.  A launch covers a list of
+// work entries: the sequences with their prefix and own keys, the sequences with their own keys only, or the prefix against all rows at
+// once.  An entry is cut into segments: a tile of `row_tile` rows (token, head of the group) of one kv head, against the key
+// tiles that any of its rows sees.  The workgroups take equal runs of the resulting units (one unit: one key tile of one
+// segment, row tiles ascending, within them the kv heads, within them the key tiles), or a segment each where there are enough of those.
 constexpr uint32_t kKeyTile = 32;
-constexpr uint32_t kTilesPerGroup = 4;      // a workgroup takes at least this many key tiles: one for each of its waves
+enum AttentionPart : uint32_t { kWholeSequences = 0, kOwnKeys = 1, kPrefix = 2 };
 
 struct AttentionArgs {
     const uint16_t* q = nullptr;
@@ -58,63 +58,110 @@ struct AttentionArgs {
     const int32_t* prefix_table = nullptr;
     const int32_t* prefix_len = nullptr;
     uint16_t* out = nullptr;
-    float* pieces = nullptr;       // two slots a workgroup: [kRowTile] max, [kRowTile] sum, [kRowTile][dim]
-    float* rows = nullptr;         // cascade: whole segments, a row of (dim + 4) a (token, head): [dim], max, sum
+    float* pieces = nullptr;       // two slots a workgroup: [row_tile] max, [row_tile] sum, [row_tile][dim]
+    float* rows = nullptr;         // not kWholeSequences: whole segments, a row of (dim + 4) a (token, head): [dim], max, sum
     uint32_t tokens = 0, sequences = 0, heads = 0, kv_heads = 0, group = 0;
     uint32_t pages = 0, page_shift = 0, pages_per_sequence = 0, prefix_pages = 0;
-    uint32_t window = 0, q_stride = 0, workgroups = 0, cascade = 0;
-    float scale_log2 = 0;          // scale * log2(e)
+    uint32_t window = 0, q_stride = 0, workgroups = 0, part = 0;
+    uint32_t row_tile = 0;
+    uint32_t least_units = 1;      // a workgroup takes at least this many units
+    uint32_t whole_from = ~0u;     // segments from which on each workgroup takes one
+    float scale_log2 = 0;          // |scale| * log2(e)
+    uint32_t flip_q = 0;           // 0x80008000 for a negative scale
 };
 
-SMELT_HD uint32_t piece_floats(uint32_t dim) { return kRowTile * (dim + 2); }
-SMELT_HD uint32_t clamp_count(int32_t v, uint32_t most) { return v < 0 ? 0u : ((uint32_t)v > most ? most : (uint32_t)v); }
+struct AttentionJoinArgs { AttentionArgs own, front; };
 
-// One work entry: rows first_row .. first_row + rows of the launch's tokens (times `group` heads), its two runs of keys.
+SMELT_HD uint32_t piece_floats(uint32_t row_tile, uint32_t dim) { return row_tile * (dim + 2); }
+SMELT_HD uint32_t clamp_count(int32_t v, uint32_t most) { return v < 0 ? 0u : ((uint32_t)v > most ? most : (uint32_t)v); }
+SMELT_HD uint32_t attention_entries(const AttentionArgs& a) { return a.part == kPrefix ? 1u : a.sequences; }
+
+// One work entry: its rows and its two runs of keys.
 struct AttentionEntry {
     uint32_t first_token = 0, tokens = 0;
     uint32_t row_tiles = 0;
+    uint32_t prefix = 0;                // prefix length, covered by this entry or not
     uint32_t front = 0, own = 0;        // keys of the prefix run and of the sequence's own run
-    uint32_t front_tiles = 0, key_tiles = 0;
+    uint32_t front_tiles = 0, tiles = 0;
     int32_t sequence = -1;              // -1: the prefix against all rows
 };
 
-SMELT_HD AttentionEntry attention_entry(const AttentionArgs& a, uint32_t index) {
+struct AttentionPlainLoad { SMELT_HD int32_t operator()(const int32_t* p, uint32_t i) const { return p[i]; } };
+template <class Load = AttentionPlainLoad>
+SMELT_HD AttentionEntry attention_entry(const AttentionArgs& a, uint32_t index, Load load = Load()) {
     AttentionEntry e;
     const uint32_t page = 1u << a.page_shift;
-    const uint32_t front = a.prefix_len ? clamp_count(a.prefix_len[0], a.prefix_pages * page) : 0u;
-    if (a.cascade && index == 0) {
-        e.tokens = clamp_count(a.offsets[a.sequences], a.tokens);
-        e.front = front;
-        e.front_tiles = e.key_tiles = (front + kKeyTile - 1) / kKeyTile;
+    e.prefix = a.prefix_len ? clamp_count(load(a.prefix_len, 0), a.prefix_pages * page) : 0u;
+    if (a.part == kPrefix) {
+        e.tokens = e.prefix ? clamp_count(load(a.offsets, a.sequences), a.tokens) : 0u;
+        e.front = e.prefix;
     } else {
-        const uint32_t s = index - a.cascade;
-        const uint32_t lo = clamp_count(a.offsets[s], a.tokens), hi = clamp_count(a.offsets[s + 1], a.tokens);
-        e.sequence = (int32_t)s;
+        const uint32_t lo = clamp_count(load(a.offsets, index), a.tokens), hi = clamp_count(load(a.offsets, index + 1), a.tokens);
+        e.sequence = (int32_t)index;
         e.first_token = lo;
         e.tokens = hi > lo ? hi - lo : 0u;
-        e.own = clamp_count(a.kv_lens[s], a.pages_per_sequence * page);
-        if (!a.cascade) e.front = front;
-        e.front_tiles = (e.front + kKeyTile - 1) / kKeyTile;
-        e.key_tiles = e.front_tiles + (e.own + kKeyTile - 1) / kKeyTile;
-        if (e.key_tiles == 0) e.key_tiles = 1;   // rows that see nothing are still written
+        e.own = clamp_count(load(a.kv_lens, index), a.pages_per_sequence * page);
+        if (a.part == kWholeSequences) e.front = e.prefix;
     }
-    e.row_tiles = (e.tokens * a.group + kRowTile - 1) / kRowTile;
+    e.front_tiles = (e.front + kKeyTile - 1) / kKeyTile;
+    e.tiles = e.front_tiles + (e.own + kKeyTile - 1) / kKeyTile;
+    e.row_tiles = (e.tokens * a.group + a.row_tile - 1) / a.row_tile;
     return e;
 }
 
-SMELT_HD uint64_t attention_units(const AttentionArgs& a, const AttentionEntry& e) { return (uint64_t)a.kv_heads * e.row_tiles * e.key_tiles; }
-SMELT_HD uint32_t attention_groups(const AttentionArgs& a, uint64_t units) {
-    const uint64_t most = (units + kTilesPerGroup - 1) / kTilesPerGroup;
-    return most < a.workgroups ? (uint32_t)most : a.workgroups;
+// Keys, counted from the prefix's first, that the rows first .. first + count of a sequence's entry see: some row those of [lo, hi), every
+// row those of [all_lo, all_hi).  (Positions stay below 2^31.)
+struct AttentionSpan { int32_t lo, hi, all_lo, all_hi; };
+SMELT_HD AttentionSpan attention_span(const AttentionArgs& a, const AttentionEntry& e, uint32_t first, uint32_t count) {
+    const int32_t zero = (int32_t)(e.prefix + e.own) - (int32_t)e.tokens;       // position of the entry's first row
+    const uint32_t last = (first + count - 1) / a.group;
+    const int32_t p0 = zero + (int32_t)(first / a.group), p1 = zero + (int32_t)(last < e.tokens ? last : e.tokens - 1);
+    AttentionSpan s{0, p1 + 1, 0, p0 + 1};
+    if (a.window) { s.lo = p0 - (int32_t)a.window + 1; s.all_lo = p1 - (int32_t)a.window + 1; }
+    return s;
 }
-// first unit of workgroup w of `groups`
-SMELT_HD uint64_t attention_start(uint64_t units, uint32_t groups, uint32_t w) { return units * w / groups; }
+
+// Key tiles lo .. hi of a row tile: those that a row of it sees, one at least (rows that see nothing are still written).
+struct AttentionTiles { uint32_t lo, hi; };
+SMELT_HD uint32_t attention_tile_of(const AttentionEntry& e, uint32_t key, uint32_t round) {   // round 0: the tile that holds a key, kKeyTile - 1: the tiles before one
+    const bool front = key < e.prefix + (round ? 1u : 0u);
+    return front ? (e.front ? (key + round) / kKeyTile : 0u) : e.front_tiles + (key - e.prefix + round) / kKeyTile;
+}
+SMELT_HD AttentionTiles attention_tiles(const AttentionArgs& a, const AttentionEntry& e, uint32_t row_tile) {
+    AttentionTiles t{0, e.tiles};
+    if (e.sequence >= 0) {
+        const AttentionSpan s = attention_span(a, e, row_tile * a.row_tile, a.row_tile);
+        t.hi = s.hi <= 0 ? 0u : attention_tile_of(e, (uint32_t)s.hi < e.prefix + e.own ? (uint32_t)s.hi : e.prefix + e.own, kKeyTile - 1);
+        if (s.lo > 0) t.lo = attention_tile_of(e, (uint32_t)s.lo, 0);
+    }
+    if (t.lo >= t.hi) { t.lo = t.lo < e.tiles ? t.lo : 0; t.hi = t.lo + 1; }
+    return t;
+}
+
+// (the host refuses shapes whose units could pass 2^31)
+SMELT_HD uint32_t attention_units(const AttentionArgs& a, const AttentionEntry& e) {
+    uint32_t n = 0;
+#pragma unroll 1
+    for (uint32_t r = 0; r < e.row_tiles; ++r) { const AttentionTiles t = attention_tiles(a, e, r); n += t.hi - t.lo; }
+    return n * a.kv_heads;
+}
+SMELT_HD uint32_t attention_segments(const AttentionArgs& a, const AttentionEntry& e) { return a.kv_heads * e.row_tiles; }
+
+// How the units fall to the launch's workgroups: runs of `each`, the first `longer` of them one longer; or a segment each.
+struct AttentionSplit { uint32_t units, groups, each, longer; bool whole; };
+SMELT_HD AttentionSplit attention_split(const AttentionArgs& a, uint32_t units, uint32_t segments) {
+    AttentionSplit s{units, 0, 0, 0, segments >= a.whole_from};
+    const uint32_t most = units / a.least_units + (units % a.least_units != 0);
+    s.groups = s.whole ? segments : (most < a.workgroups ? most : a.workgroups);
+    if (s.groups) { s.each = units / s.groups; s.longer = units - s.each * s.groups; }
+    return s;
+}
+// first unit of workgroup w
+SMELT_HD uint32_t attention_start(const AttentionSplit& s, uint32_t w) { return w * s.each + (w < s.longer ? w : s.longer); }
 // the workgroup whose run holds unit u
-SMELT_HD uint32_t attention_owner(uint64_t units, uint32_t groups, uint64_t u) {
-    uint32_t w = (uint32_t)(u * groups / units);
-    while (w + 1 < groups && attention_start(units, groups, w + 1) <= u) ++w;
-    while (w > 0 && attention_start(units, groups, w) > u) --w;
-    return w;
+SMELT_HD uint32_t attention_owner(const AttentionSplit& s, uint32_t u) {
+    const uint32_t border = s.longer * (s.each + 1);
+    return u < border ? u / (s.each + 1) : s.longer + (u - border) / s.each;
 }
 
 // ---- verification of drafted tokens ----------------------------------------------------------------------------------

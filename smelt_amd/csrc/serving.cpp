@@ -1,6 +1,7 @@
 // Serving operators on the host: pipeline names, argument checks, launch plans.  No device is touched here.
 #include "serving.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -11,6 +12,8 @@ namespace smelt_host {
 using namespace smelt_serving;
 
 namespace {
+
+constexpr uint32_t kStreamRows = 32;     // row tile of the streaming attention kernel
 
 // "_d256" at `at`: the number behind the letters, and the position behind it
 bool number_after(const std::string& s, const char* letters, size_t* at, uint32_t* out) {
@@ -81,7 +84,8 @@ ResolveStatus resolve_serving(const std::string& entry, const char* act, Resolve
         out->appended = {dim, heads, kv_heads, page};
         const std::string d = "d" + std::to_string(dim);
         const std::string small = page == 16 ? "_p16" : "";
-        out->serving_symbols = {"smelt_attention_stream_" + d + small + t, "smelt_attention_join_" + d + t};
+        out->serving_symbols = {"smelt_attention_stream_" + d + small + t, "smelt_attention_tiles_" + d + small + t, "smelt_attention_join_" + d + t,
+                                "smelt_attention_join_shared_" + d + t};
         out->symbol = out->serving_symbols[0];
         return kResolveOk;
     }
@@ -253,7 +257,9 @@ int Planner::attention() {
     if ((uint64_t)a.tokens * a.heads > 0x7FFFFFFFull) return bad("more than 2^31 - 1 rows");
     if (a.q_stride < a.heads * dim) return bad("q's row stride is shorter than its heads");
     if (!std::isfinite(scale)) return bad("the scale must be finite");
-    a.scale_log2 = scale * 1.4426950408889634f;
+    // (a scale of zero weighs every key alike; the smallest normal number does the same and keeps a hidden key's -inf one)
+    a.scale_log2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 1.2e-38f);
+    a.flip_q = scale < 0.0f ? 0x80008000u : 0u;
     const size_t cache = (size_t)a.pages * page * a.kv_heads * dim * 2;
     need(0, row_bytes(a.tokens, a.heads * dim, a.q_stride));
     need(1, cache, 16);
@@ -272,21 +278,64 @@ int Planner::attention() {
     a.out = P<uint16_t>(6);
     if (shared && a.prefix_pages) { a.prefix_table = P<int32_t>(7); a.prefix_len = P<int32_t>(8); }
 
-    // The parts of cut segments live in the context's workspace: two a workgroup, and in a cascade two rows for each row.
-    const size_t slot = (size_t)piece_floats(dim) * 4 * 2;
-    const uint32_t resident = dev.compute_units * (dim == 256 ? 1u : 2u);
-    a.workgroups = resident;
-    const size_t row_region = (size_t)2 * a.tokens * a.heads * (dim + 4) * 4;
-    a.cascade = shared && a.prefix_pages && row_region + slot <= dev.workspace_bytes ? 1u : 0u;
-    const size_t left = dev.workspace_bytes - (a.cascade ? row_region : 0);
-    if (left < slot) return bad("the workspace holds no part of a segment");
-    if ((size_t)a.workgroups * slot > left) a.workgroups = (uint32_t)(left / slot);
-    a.rows = static_cast<float*>(dev.workspace);
-    a.pieces = reinterpret_cast<float*>(static_cast<char*>(dev.workspace) + (a.cascade ? row_region : 0));
-    // LDS: the four waves' results (rows padded by four floats), their maxima and sums, the partition's scratch
-    const size_t lds = (size_t)4 * 32 * (dim + 4) * 4 + 2 * 4 * 32 * 4 + 16 * 8;
-    step(0, a, a.workgroups, 1, 1, 256, lds);
-    step(1, a, a.tokens, a.kv_heads, 1, 256, 0);
+    // The streaming kernel takes the sequences while they have few rows each (one row tile on average), the prefix then being read once
+    // against all rows; the tile kernel takes longer runs of rows, whose tiles read prefix and own keys alike.
+    const uint64_t rows = (uint64_t)a.tokens * a.group;
+    const bool stream = rows <= (uint64_t)kStreamRows * a.sequences;
+    const uint32_t tile_rows = dim == 256 ? 128 : 256;
+    // The parts of cut segments live in the context's workspace: two a workgroup; with the prefix apart, so do the rows
+    // of segments that one workgroup finished.
+    auto slot_bytes = [&](uint32_t row_tile) { return (size_t)piece_floats(row_tile, dim) * 4 * 2; };
+    const size_t row_region = (size_t)a.tokens * a.heads * (dim + 4) * 4;
+    char* ws = static_cast<char*>(dev.workspace);
+    auto lay_out = [&](AttentionArgs& x, bool streams, size_t room) {
+        x.row_tile = streams ? kStreamRows : tile_rows;
+        x.least_units = streams ? 4 : 8;       // a key tile for each of four waves; two stages
+        const uint32_t resident = dev.compute_units * (streams && dim != 256 ? 2u : 1u);
+        x.workgroups = (uint32_t)std::min<size_t>(resident, room / slot_bytes(x.row_tile));
+        // a segment each from three quarters of the workgroups on: no parts to write and join
+        x.whole_from = streams ? ~0u : std::max(1u, dev.compute_units * 3 / 4);
+    };
+    auto main_step = [&](const AttentionArgs& x, bool streams) {
+        const size_t lds = streams ? (size_t)4 * 32 * (dim + 4) * 4 + 2 * 4 * 32 * 4 : (size_t)2 * 2 * (dim == 256 ? 1 : 2) * 32 * dim * 2;
+        uint32_t grid = x.workgroups;
+        if (!streams) {      // as many as there can be segments
+            const uint64_t entry_rows = (uint64_t)x.tokens * x.group, most = ((entry_rows + x.row_tile - 1) / x.row_tile + (x.part == kPrefix ? 0 : x.sequences)) * x.kv_heads;
+            grid = (uint32_t)std::max<uint64_t>(grid, std::min<uint64_t>(most, 0x7FFFFFFFull));
+        }
+        step(streams ? 0 : 1, x, grid, 1, 1, streams || dim == 256 ? 256 : 512, lds);
+    };
+    // units are counted in 32 bits
+    const uint64_t key_tiles = ((uint64_t)a.pages_per_sequence + a.prefix_pages) * page / kKeyTile + 2;
+    const uint64_t row_tiles = rows / (stream ? kStreamRows : tile_rows) + a.sequences + 1;
+    if (row_tiles * a.kv_heads > 0x7FFFFFFFull / key_tiles) return bad("rows times keys pass 2^31 key tiles");
+    const bool prefix = shared && a.prefix_pages;
+    if (stream && prefix && 2 * row_region + slot_bytes(kStreamRows) + slot_bytes(tile_rows) <= dev.workspace_bytes) {
+        const bool front_streams = rows <= kStreamRows;
+        AttentionJoinArgs both;
+        both.front = a; both.own = a;
+        both.front.part = kPrefix; both.own.part = kOwnKeys;
+        both.front.rows = reinterpret_cast<float*>(ws);
+        both.own.rows = reinterpret_cast<float*>(ws + row_region);
+        const size_t room = dev.workspace_bytes - 2 * row_region;
+        lay_out(both.own, true, room / 2);
+        const size_t own_bytes = (size_t)both.own.workgroups * slot_bytes(kStreamRows);
+        lay_out(both.front, front_streams, room - own_bytes);
+        if (both.own.workgroups && both.front.workgroups) {
+            both.own.pieces = reinterpret_cast<float*>(ws + 2 * row_region);
+            both.front.pieces = reinterpret_cast<float*>(ws + 2 * row_region + own_bytes);
+            main_step(both.front, front_streams);
+            main_step(both.own, true);
+            step(3, both, a.tokens, a.kv_heads, 1, 256, 0);
+            return 0;
+        }
+    }
+    a.part = kWholeSequences;
+    a.pieces = reinterpret_cast<float*>(ws);
+    lay_out(a, stream, dev.workspace_bytes);
+    if (a.workgroups == 0) return bad("the workspace holds no part of a segment");
+    main_step(a, stream);
+    if (a.workgroups > 1) step(2, a, a.workgroups - 1, stream ? 2 : 8, 1, 256, 0);
     return 0;
 }
 

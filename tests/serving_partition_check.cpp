@@ -7,33 +7,43 @@ using namespace smelt_serving;
 
 extern "C" {
 
-// entry: {first_token, tokens, row_tiles, front, own, front_tiles, key_tiles, sequence}; returns the entry count
+// entry: {first_token, tokens, row_tiles, front, own, front_tiles, tiles, sequence}; tiles: {lo, hi} of each row tile of each entry, in
+// order; returns the entry count
 int check_entries(const int32_t* offsets, const int32_t* lens, int sequences, int tokens, int group, int kv_heads, int page_shift,
-                  int pages_per_sequence, const int32_t* prefix_len, int prefix_pages, int cascade, int64_t* out, uint64_t* units) {
+                  int pages_per_sequence, const int32_t* prefix_len, int prefix_pages, int part, int row_tile, int window, int64_t* out,
+                  int64_t* tiles, uint64_t* units) {
     AttentionArgs a;
     a.offsets = offsets; a.kv_lens = lens; a.sequences = sequences; a.tokens = tokens; a.group = group; a.kv_heads = kv_heads;
-    a.page_shift = page_shift; a.pages_per_sequence = pages_per_sequence; a.prefix_len = prefix_len; a.prefix_pages = prefix_pages; a.cascade = cascade;
+    a.page_shift = page_shift; a.pages_per_sequence = pages_per_sequence; a.prefix_len = prefix_len; a.prefix_pages = prefix_pages;
+    a.part = part; a.row_tile = row_tile; a.window = window;
     uint64_t total = 0;
-    for (int i = 0; i < sequences + cascade; ++i) {
+    const int n = (int)attention_entries(a);
+    for (int i = 0; i < n; ++i) {
         const AttentionEntry e = attention_entry(a, i);
-        const int64_t f[8] = {e.first_token, e.tokens, e.row_tiles, e.front, e.own, e.front_tiles, e.key_tiles, e.sequence};
+        const int64_t f[8] = {e.first_token, e.tokens, e.row_tiles, e.front, e.own, e.front_tiles, e.tiles, e.sequence};
         for (int k = 0; k < 8; ++k) out[8 * i + k] = f[k];
+        for (uint32_t r = 0; r < e.row_tiles; ++r) {
+            const AttentionTiles t = attention_tiles(a, e, r);
+            *tiles++ = t.lo;
+            *tiles++ = t.hi;
+        }
         total += attention_units(a, e);
     }
     *units = total;
-    return sequences + cascade;
+    return n;
 }
 
 // every unit has one owner, owners are in order, and the owner's run holds the unit; 0 or the first bad unit + 1
-uint64_t check_owners(uint64_t units, uint32_t workgroups) {
+uint64_t check_owners(uint32_t units, uint32_t workgroups, uint32_t least) {
     AttentionArgs a;
     a.workgroups = workgroups;
-    const uint32_t groups = attention_groups(a, units);
-    if (groups == 0 || groups > workgroups) return 1;
-    if (attention_start(units, groups, 0) != 0 || attention_start(units, groups, groups) != units) return 1;
-    for (uint64_t u = 0; u < units; ++u) {
-        const uint32_t w = attention_owner(units, groups, u);
-        if (w >= groups || attention_start(units, groups, w) > u || attention_start(units, groups, w + 1) <= u) return u + 1;
+    a.least_units = least;
+    const AttentionSplit s = attention_split(a, units, 1);
+    if (s.groups == 0 || s.groups > workgroups || s.whole) return 1;
+    if (attention_start(s, 0) != 0 || attention_start(s, s.groups) != units) return 1;
+    for (uint32_t u = 0; u < units; ++u) {
+        const uint32_t w = attention_owner(s, u);
+        if (w >= s.groups || attention_start(s, w) > u || attention_start(s, w + 1) <= u) return (uint64_t)u + 1;
     }
     return 0;
 }

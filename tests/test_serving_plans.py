@@ -181,41 +181,77 @@ def partition(tmp_path_factory):
     subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-o", out, os.path.join(HERE, "serving_partition_check.cpp")], check=True)
     lib = C.CDLL(out)
     lib.check_owners.restype = C.c_uint64
-    lib.check_owners.argtypes = [C.c_uint64, C.c_uint32]
+    lib.check_owners.argtypes = [C.c_uint32, C.c_uint32, C.c_uint32]
     return lib
 
 
-def entries(lib, offsets, lens, tokens, group=1, kv_heads=1, shift=4, width=4, prefix=None, prefix_pages=0, cascade=0):
+WHOLE, OWN, PREFIX = range(3)
+
+
+def entries(lib, offsets, lens, tokens, group=1, kv_heads=1, shift=4, width=4, prefix=None, prefix_pages=0, part=WHOLE, row_tile=32, window=0):
     offsets, lens = np.array(offsets, np.int32), np.array(lens, np.int32)
-    out, units = np.zeros((len(lens) + 1, 8), np.int64), C.c_uint64()
+    out, tiles, units = np.zeros((len(lens) + 1, 8), np.int64), np.zeros((100000, 2), np.int64), C.c_uint64()
     p = None if prefix is None else C.byref(C.c_int32(prefix))
-    i32p = C.POINTER(C.c_int32)
-    n = lib.check_entries(offsets.ctypes.data_as(i32p), lens.ctypes.data_as(i32p), len(lens), tokens, group, kv_heads, shift, width, p, prefix_pages, cascade,
-                          out.ctypes.data_as(C.POINTER(C.c_int64)), C.byref(units))
-    keys = ("first", "tokens", "row_tiles", "front", "own", "front_tiles", "key_tiles", "sequence")
-    return [dict(zip(keys, r)) for r in out[:n].tolist()], units.value
+    i32p, i64p = C.POINTER(C.c_int32), C.POINTER(C.c_int64)
+    n = lib.check_entries(offsets.ctypes.data_as(i32p), lens.ctypes.data_as(i32p), len(lens), tokens, group, kv_heads, shift, width, p, prefix_pages, part, row_tile, window,
+                          out.ctypes.data_as(i64p), tiles.ctypes.data_as(i64p), C.byref(units))
+    keys = ("first", "tokens", "row_tiles", "front", "own", "front_tiles", "tiles", "sequence")
+    got = [dict(zip(keys, r)) for r in out[:n].tolist()]
+    at = 0
+    for e in got:
+        e["of_rows"] = [tuple(t) for t in tiles[at:at + e["row_tiles"]].tolist()]
+        at += e["row_tiles"]
+    assert units.value == kv_heads * sum(hi - lo for e in got for lo, hi in e["of_rows"])
+    return got
 
 
 def test_entries_are_cut_to_what_the_tables_hold(partition):
     # lengths past the table, negative lengths, offsets outside the rows or falling
-    e, units = entries(partition, [0, 3, 3, -5, 900], [1000, 7, -4, 64], tokens=10, group=12, kv_heads=2)
+    e = entries(partition, [0, 3, 3, -5, 900], [1000, 7, -4, 64], tokens=10, group=12, kv_heads=2)
     assert [x["own"] for x in e] == [64, 7, 0, 64] and [x["tokens"] for x in e] == [3, 0, 0, 10]
-    assert [x["first"] for x in e] == [0, 3, 3, 0] and [x["key_tiles"] for x in e] == [2, 1, 1, 2] and [x["row_tiles"] for x in e] == [2, 0, 0, 4]
-    assert units == 2 * (2 * 2 + 4 * 2)
+    assert [x["first"] for x in e] == [0, 3, 3, 0] and [x["tiles"] for x in e] == [2, 1, 0, 2] and [x["row_tiles"] for x in e] == [2, 0, 0, 4]
     # a prefix longer than its table; the prefix entry covers the rows that belong to a sequence
-    e, units = entries(partition, [0, 1, 2], [5, 0], tokens=4, prefix=1 << 30, prefix_pages=3, cascade=1)
-    assert e[0] == dict(first=0, tokens=2, row_tiles=1, front=48, own=0, front_tiles=2, key_tiles=2, sequence=-1)
-    assert [x["key_tiles"] for x in e[1:]] == [1, 1] and units == 2 + 1 + 1
-    e, _ = entries(partition, [0, 1], [0], tokens=4, prefix=-3, prefix_pages=3, cascade=1)
-    assert e[0]["key_tiles"] == 0 and e[1]["key_tiles"] == 1
-    e, _ = entries(partition, [0, 1], [33], tokens=4, prefix=40, prefix_pages=3)
-    assert (e[0]["front_tiles"], e[0]["key_tiles"]) == (2, 4)
+    e = entries(partition, [0, 1, 2], [5, 0], tokens=4, prefix=1 << 30, prefix_pages=3, part=PREFIX)
+    assert len(e) == 1 and {k: e[0][k] for k in ("first", "tokens", "row_tiles", "front", "own", "tiles", "sequence")} == dict(
+        first=0, tokens=2, row_tiles=1, front=48, own=0, tiles=2, sequence=-1)
+    assert e[0]["of_rows"] == [(0, 2)]
+    e = entries(partition, [0, 1, 2], [5, 0], tokens=4, prefix=1 << 30, prefix_pages=3, part=OWN)
+    assert [x["tiles"] for x in e] == [1, 0] and [x["of_rows"] for x in e] == [[(0, 1)], [(0, 1)]]     # (rows without keys are still written)
+    assert entries(partition, [0, 1], [0], tokens=4, prefix=-3, prefix_pages=3, part=PREFIX)[0]["row_tiles"] == 0
+    e = entries(partition, [0, 1], [33], tokens=4, prefix=40, prefix_pages=3)
+    assert (e[0]["front_tiles"], e[0]["tiles"]) == (2, 4)
+
+
+@pytest.mark.parametrize("part", [WHOLE, OWN])
+@pytest.mark.parametrize("prefix", [0, 1, 31, 32, 33, 100])
+@pytest.mark.parametrize("window", [0, 1, 30, 64, 1000])
+def test_row_tiles_cover_what_their_rows_see(partition, part, prefix, window):
+    """Against the definition, key by key: the key tiles of a row tile are the smallest run that holds every key one of its rows sees."""
+    for n, own, group, row_tile in ((1, 1, 1, 32), (1, 100, 6, 32), (70, 70, 1, 32), (70, 200, 3, 128), (40, 33, 2, 32), (9, 0, 4, 32), (300, 310, 4, 256)):
+        e = entries(partition, [0, n], [own], tokens=n, group=group, width=64, prefix=prefix, prefix_pages=7, part=part, row_tile=row_tile, window=window)[0]
+        assert e["row_tiles"] == -(-n * group // row_tile)
+        front = prefix if part == WHOLE else 0
+        tile_of = [j // 32 for j in range(front)] + [-(-front // 32) + j // 32 for j in range(own)]
+        for r, (lo, hi) in enumerate(e["of_rows"]):
+            seen = set()
+            for row in range(r * row_tile, min((r + 1) * row_tile, n * group)):
+                p = prefix + own - n + row // group
+                for k, t in enumerate(tile_of):
+                    j = k if part == WHOLE else prefix + k
+                    if j <= p and (not window or j > p - window):
+                        seen.add(t)
+            assert hi > lo >= 0
+            if seen:
+                assert (lo, hi) == (min(seen), max(seen) + 1), (n, own, group, row_tile, r)
+            else:
+                assert hi - lo == 1 and (lo < max(e["tiles"], 1))
 
 
 def test_every_unit_has_one_workgroup(partition):
     for units in (1, 2, 3, 4, 5, 63, 64, 1000, 1021, 4096, 100003):
         for workgroups in (1, 2, 7, 256, 512):
-            assert partition.check_owners(units, workgroups) == 0, (units, workgroups)
+            for least in (1, 4):
+                assert partition.check_owners(units, workgroups, least) == 0, (units, workgroups, least)
 
 
 def test_reciprocal_division_is_exact(partition):
