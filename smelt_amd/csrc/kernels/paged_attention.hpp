@@ -146,9 +146,10 @@ __device__ __forceinline__ AttnWork find_work(const AttentionArgs& a, uint32_t w
 struct AttnSegment {
     uint32_t kv_head, row_tile;
     AttentionTiles tiles;        // the segment's
-    uint32_t first, last;        // the workgroup's part of them
+    uint32_t first, last;        // the workgroup's part of them (none when its run ends within the segment's lead)
     bool whole;
-    uint32_t begin;              // the segment's first unit
+    uint32_t begin;              // the unit of the segment's first key tile
+    uint32_t units;              // of the workgroup's run that lie in the segment
 };
 // the segment that holds unit `unit` of entry e, whose units start at `base`; false (and g.begin behind them) when the entry has fewer
 __device__ __forceinline__ bool attn_segment(const AttentionArgs& a, const AttentionEntry& e, uint32_t base, uint32_t unit, uint32_t unit_end, AttnSegment& g) {
@@ -157,14 +158,15 @@ __device__ __forceinline__ bool attn_segment(const AttentionArgs& a, const Atten
 #pragma unroll 1
     for (g.row_tile = 0; g.row_tile < e.row_tiles; ++g.row_tile) {
         g.tiles = smelt_serving::attention_tiles(a, e, g.row_tile);
-        const uint32_t tiles = g.tiles.hi - g.tiles.lo, size = tiles * a.kv_heads;
+        const uint32_t each = g.tiles.hi - g.tiles.lo + a.lead, size = each * a.kv_heads;
         if (rel >= size) { rel -= size; g.begin += size; continue; }
-        g.kv_head = rel / tiles;
-        const uint32_t done = rel - g.kv_head * tiles;
-        g.begin += g.kv_head * tiles;
-        g.first = g.tiles.lo + done;
-        g.last = tiles - done < unit_end - unit ? g.tiles.hi : g.first + (unit_end - unit);
-        g.whole = done == 0 && g.last == g.tiles.hi;
+        g.kv_head = rel / each;
+        const uint32_t done = rel - g.kv_head * each, left = each - done;
+        g.begin += g.kv_head * each + a.lead;
+        g.units = left < unit_end - unit ? left : unit_end - unit;
+        g.first = g.tiles.lo + (done > a.lead ? done - a.lead : 0u);
+        g.last = g.tiles.lo + (done + g.units > a.lead ? done + g.units - a.lead : 0u);
+        g.whole = g.first == g.tiles.lo && g.last == g.tiles.hi;
         return true;
     }
     return false;
@@ -178,6 +180,7 @@ __device__ __forceinline__ void attn_whole_segment(const AttentionArgs& a, const
     g.last = g.tiles.hi;
     g.whole = true;
     g.begin = 0;
+    g.units = 1;
 }
 
 // the sequence of a token row: offsets is ascending, tokens before offsets[sequences] belong to one
@@ -227,24 +230,22 @@ __device__ __forceinline__ AttnBounds attn_bounds(const AttentionArgs& a, const 
     return b;
 }
 
-// Keys of one run that some row of a wave sees, and that all of its rows see.
-struct AttnRun { int32_t len, lo, hi, all_lo, all_hi; };
-__device__ __forceinline__ AttnRun attn_run(const AttentionArgs& a, const AttentionEntry& e, int run, uint32_t row0, const AttnRow& row) {
-    AttnRun u;
-    u.len = (int32_t)(run ? e.own : e.front);
-    u.lo = u.all_lo = 0;
-    u.hi = u.all_hi = u.len;
-    const int32_t base = run ? (int32_t)e.prefix : 0;
+// Keys of one run that some of `count` rows from row0 on sees, and that all of them see (b: the lane's own).
+struct AttnRun { int32_t lo, hi, all_lo, all_hi; };
+__device__ __forceinline__ AttnRun attn_run(const AttentionArgs& a, const AttentionEntry& e, int run, uint32_t row0, uint32_t count, const AttnBounds* b, int bounds) {
+    const int32_t len = (int32_t)(run ? e.own : e.front), base = run ? (int32_t)e.prefix : 0;
+    AttnRun u{0, len, 0, len};
     if (e.sequence < 0) {        // rows of many sequences: they mostly see all of it
-        const AttnBounds b = attn_bounds(a, row, 0, u.len);
-        if (__any(b.lo != 0 || b.hi != u.len)) u.all_hi = 0;
+        bool all = true;
+        for (int t = 0; t < bounds; ++t) all = all && b[t].lo == 0 && b[t].hi == len;
+        if (!__all(all)) u.all_hi = 0;
     } else if (row0 < e.tokens * a.group) {
-        const AttentionSpan s = smelt_serving::attention_span(a, e, row0, 32);
+        const AttentionSpan s = smelt_serving::attention_span(a, e, row0, count);
         const int32_t hi = s.hi - base, all_hi = s.all_hi - base;
         u.lo = s.lo - base > 0 ? s.lo - base : 0;
         u.all_lo = s.all_lo - base > 0 ? s.all_lo - base : 0;
-        u.hi = hi < u.len ? hi : u.len;
-        u.all_hi = all_hi < u.len ? all_hi : u.len;
+        u.hi = hi < len ? hi : len;
+        u.all_hi = all_hi < len ? all_hi : len;
     } else {
         u.hi = 0;                // no rows here
     }
@@ -260,89 +261,48 @@ struct AttnAcc {
     float m, l;              // running maximum of q.k and this half's sum
 };
 
-template <class ActT, int D>
-__device__ __forceinline__ void attn_load_q(const AttentionArgs& a, const AttnRow& r, uint32_t kv_head, uint4_t* qf) {
-    const int half = (threadIdx.x & 63) >> 5;
-    const uint16_t* q = a.q + (size_t)r.token * a.q_stride + (size_t)(kv_head * a.group + r.head) * D + 8 * half;
+// N pieces of eight values of a q row, `step` apart; rows that are none (they point at a row that is one) are zero
+template <int N>
+__device__ __forceinline__ void attn_load_q(const AttentionArgs& a, const AttnRow& r, const uint16_t* q, uint32_t step, uint4_t* qf) {
     if ((reinterpret_cast<uintptr_t>(a.q) & 15u) == 0 && (a.q_stride & 7u) == 0) {
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) qf[t] = r.live ? *reinterpret_cast<const uint4_t*>(q + 16 * t) ^ a.flip_q : uint4_t{0, 0, 0, 0};
+        for (int k = 0; k < N; ++k) qf[k] = *reinterpret_cast<const uint4_t*>(q + k * step);
     } else {
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) {
+        for (int k = 0; k < N; ++k) {
             uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = r.live ? (uint32_t)q[16 * t + 2 * k] | ((uint32_t)q[16 * t + 2 * k + 1] << 16) : 0u;
-            qf[t] = uint4_t{w[0], w[1], w[2], w[3]} ^ a.flip_q;
+            for (int i = 0; i < 4; ++i) w[i] = (uint32_t)q[k * step + 2 * i] | ((uint32_t)q[k * step + 2 * i + 1] << 16);
+            qf[k] = uint4_t{w[0], w[1], w[2], w[3]};
         }
     }
+#pragma unroll
+    for (int k = 0; k < N; ++k) qf[k] = r.live ? qf[k] ^ a.flip_q : uint4_t{0, 0, 0, 0};
 }
 
-// Address of one key tile: the page (two for pages of 16) and whether it is one of the pool's.
-template <bool SMALL>
+// Address of one key tile, in halves of 16 keys (a page holds one at least): where each lies and whether its page is one of the pool's.
 struct AttnTile {
-    size_t base[SMALL ? 2 : 1];      // element offset of the page's head
-    uint32_t known;                  // bits 0 and 1: the pages of the tile's halves are the pool's
-    uint32_t off;                    // first key within the page
+    size_t page[2];                  // element offset of the page's head
+    uint32_t off[2];                 // first key within the page
+    uint32_t known;                  // bits 0 and 1
 };
-
-template <bool SMALL, int D>
-__device__ __forceinline__ AttnTile<SMALL> attn_tile(const AttentionArgs& a, const int32_t* table, uint32_t kv_head, uint32_t run_len, uint32_t tile) {
-    AttnTile<SMALL> t;
-    const uint32_t key = tile * smelt_serving::kKeyTile;
+template <int D>
+__device__ __forceinline__ AttnTile attn_tile(const AttentionArgs& a, const int32_t* table, uint32_t kv_head, uint32_t run_len, uint32_t tile) {
+    AttnTile t;
     const uint32_t last_page = run_len ? (run_len - 1) >> a.page_shift : 0u;
     t.known = 0;
-    t.off = SMALL ? 0u : key & ((1u << a.page_shift) - 1u);
 #pragma unroll
-    for (int k = 0; k < (SMALL ? 2 : 1); ++k) {
-        uint32_t index = (key >> a.page_shift) + k;
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t key = tile * smelt_serving::kKeyTile + 16 * k;
+        uint32_t index = key >> a.page_shift;
         if (index > last_page) index = last_page;      // behind the run: masked by its length
         const uint32_t page = (uint32_t)as_scalar(table)[__builtin_amdgcn_readfirstlane(index)];
         const bool known = page < a.pages;
-        t.known |= known ? (SMALL ? 1u << k : 3u) : 0u;
-        t.base[k] = (((size_t)(known ? page : 0u) * a.kv_heads + kv_head) * D) << a.page_shift;
+        t.known |= known ? 1u << k : 0u;
+        t.page[k] = (((size_t)(known ? page : 0u) * a.kv_heads + kv_head) * D) << a.page_shift;
+        t.off[k] = key & ((1u << a.page_shift) - 1u);
     }
     return t;
-}
-
-template <int D, bool SMALL>
-__device__ __forceinline__ void attn_load_k(const AttentionArgs& a, const AttnTile<SMALL>& t, uint4_t* kf) {
-    const uint32_t lane = threadIdx.x & 63, half = lane >> 5, key = lane & 31;
-    const uint16_t* base;
-    uint32_t at;
-    if (SMALL) { base = a.k_cache + (key < 16 ? t.base[0] : t.base[SMALL ? 1 : 0]); at = key & 15; }
-    else { base = a.k_cache + t.base[0]; at = t.off + key; }
-    const uint32_t lane_off = ((half << a.page_shift) + at) * 8;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) kf[s] = *reinterpret_cast<const uint4_t*>(base + lane_off + ((uint32_t)(2 * s) << a.page_shift) * 8);
-}
-
-// D / 32 neighbouring values of 16 keys: vf[u][r] is key 16 u + 8 (r / 4) + 4 half + r % 4 of the tile
-template <int D>
-struct AttnV { uint32_t w[2][8][D / 64]; };
-
-template <int D, bool SMALL>
-__device__ __forceinline__ void attn_load_v(const AttentionArgs& a, const AttnTile<SMALL>& t, AttnV<D>& vf) {
-    const uint32_t lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const uint32_t key = 8 * (r / 4) + 4 * half + (r % 4) + (SMALL ? 0u : 16 * u + t.off);
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(a.v_cache + t.base[SMALL ? u : 0] + key * D) + col * (D / 64);
-            if constexpr (D == 256) { const uint4_t v = *reinterpret_cast<const uint4_t*>(src); vf.w[u][r][0] = v.x; vf.w[u][r][1] = v.y; vf.w[u][r][2] = v.z; vf.w[u][r][3] = v.w; }
-            else if constexpr (D == 128) { const uint2_t v = *reinterpret_cast<const uint2_t*>(src); vf.w[u][r][0] = v.x; vf.w[u][r][1] = v.y; }
-            else vf.w[u][r][0] = *src;
-        }
-}
-
-// one key tile: scores, running maximum and sum, second product
-template <class ActT, int D, bool SMALL>
-__device__ __forceinline__ void attn_scores(const AttentionArgs& a, const uint4_t* qf, const uint4_t* kf, float16_t& s) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < D / 16; ++t) s = attn_mfma<ActT>(kf[t], qf[t], s);
 }
 
 // scores of NS key tiles to probabilities: the running maximum and sum move on; s becomes p
@@ -396,39 +356,6 @@ __device__ __forceinline__ uint4_t attn_pack(const float16_t& p, int u) {
                    attn_pack2<ActT>(p[8 * u + 6], p[8 * u + 7])};
 }
 
-template <class ActT, int D>
-__device__ __forceinline__ void attn_values(AttnAcc<D>& acc, const float16_t& p, const AttnV<D>& vf) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const uint4_t pf = attn_pack<ActT>(p, u);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-            uint4_t v;
-            v.x = __builtin_amdgcn_perm(vf.w[u][1][j / 2], vf.w[u][0][j / 2], sel);
-            v.y = __builtin_amdgcn_perm(vf.w[u][3][j / 2], vf.w[u][2][j / 2], sel);
-            v.z = __builtin_amdgcn_perm(vf.w[u][5][j / 2], vf.w[u][4][j / 2], sel);
-            v.w = __builtin_amdgcn_perm(vf.w[u][7][j / 2], vf.w[u][6][j / 2], sel);
-            acc.o[j] = attn_mfma<ActT>(v, pf, acc.o[j]);
-        }
-    }
-}
-
-// Values of keys behind the run's end (or on a page that is none of the pool's) are whatever memory holds: zero them, since a zero
-// probability does not silence an infinity or a NaN.
-template <int D, bool SMALL>
-__device__ __forceinline__ void attn_clear_v(AttnV<D>& vf, const AttnTile<SMALL>& t, int32_t key0, int32_t run_len) {
-    const int half = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const bool ok = key0 + 16 * u + 8 * (r / 4) + 4 * half + r % 4 < run_len && ((t.known >> u) & 1u);
-#pragma unroll
-            for (int k = 0; k < D / 64; ++k) vf.w[u][r][k] = ok ? vf.w[u][r][k] : 0u;
-        }
-}
-
 // Where the finished rows of a segment go that are not the whole answer (kOwnKeys, kPrefix).
 __device__ __forceinline__ float* attn_whole_row(const AttentionArgs& a, uint32_t token, uint32_t head, uint32_t dim) {
     return a.rows + ((size_t)token * a.heads + head) * (dim + 4);
@@ -444,91 +371,200 @@ __device__ __forceinline__ void attn_clear(AttnAcc<D>& acc) {
         for (int i = 0; i < 16; ++i) acc.o[j][i] = 0.0f;
 }
 
+// maximum and sum over a lane's row of the streaming kernel: lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float attn_quarters_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return attn_halves_max(__builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1])));
+}
+__device__ __forceinline__ float attn_quarters_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return attn_halves_sum(__builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+template <class ActT>
+__device__ __forceinline__ float4_t attn_mfma16(uint4_t a, uint4_t b, float4_t c) {
+    if constexpr (ActT::kIsF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(attn_bf16x8_t, a), __builtin_bit_cast(attn_bf16x8_t, b), c, 0, 0, 0);
+}
+
 // LDS of the streaming kernel: partial outputs of the four waves, their maxima and sums
-template <int D>
+template <int D, int RT>
 struct AttnShared {
-    float o[4][32][D + 4];      // (four floats of padding: a half wave's 16-byte stores cover all banks)
-    float m[4][32], l[4][32];
+    float o[4][16 * RT][D + 4];      // (four floats of padding: neighbouring rows' 16-byte stores lie on different banks)
+    float m[4][16 * RT], l[4][16 * RT];
 };
 
 // Few rows a sequence (decoding, drafted tokens): bound by the cache's bytes.  A workgroup takes a run of units and works
-// through the segments it crosses, its four waves on every fourth key tile, straight from the cache: a lane takes dim / 32 neighbouring
-// values of 16 keys of V, and pairs of keys are put side by side with one v_perm per operand dword.  At a segment's end the
-// waves' results meet in LDS.  A segment that lies whole in one workgroup is finished there; the parts of the others go to the workspace
-// (two slots a workgroup are enough: only its first and last segment can be shared) and are joined by the second launch, in a
-// fixed order.
-template <class ActT, int D, bool SMALL>
+// through the segments it crosses, its four waves on every fourth key tile, straight from the cache.  Here the products are
+// v_mfma_f32_16x16x32 (lane l: row l % 16, quarter l / 16), one or two tiles of 16 rows against each key tile: with one, heads of
+// 256 leave room for two workgroups a compute unit, whose starts and ends hide behind each other.  V: a lane takes 8 neighbouring
+// values (4 for heads of 64) of the 8 keys whose probabilities it holds, and pairs of keys are put side by side with one
+// v_perm per operand dword.  At a segment's end the waves' results meet in LDS.  A segment that lies whole in one workgroup is
+// finished there; the parts of the others go to the workspace (two slots a workgroup are enough: only its first and last segment can be
+// shared) and are joined by the second launch, in a fixed order.
+template <class ActT, int D, int RT>
 __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    AttnShared<D>& sh = *reinterpret_cast<AttnShared<D>*>(smem);
-    constexpr uint32_t R = 32;
+    AttnShared<D, RT>& sh = *reinterpret_cast<AttnShared<D, RT>*>(smem);
+    constexpr uint32_t R = 16 * RT;
+    constexpr int KS = D / 32, VE = D == 64 ? 4 : 8, VC = D == 256 ? 2 : 1, MT = D / 16;   // k steps of a score; values a lane takes of a V row, in VC pieces; tiles of 16 values
     const AttnWork work = find_work<kFirstUnit>(a, blockIdx.x);
     if (work.entry == ~0u) return;
     uint32_t unit = work.at, index = work.entry, base = work.base;
     const uint32_t unit_end = smelt_serving::attention_start(work.split, blockIdx.x + 1);
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, quarter = lane >> 4, col = lane & 15;
     const AttnScale scale = attn_scale(a);
 #pragma unroll 1
     while (unit < unit_end) {
         const AttentionEntry e = attn_entry(a, index);
         AttnSegment g;
         if (!attn_segment(a, e, base, unit, unit_end, g)) { base = g.begin; ++index; continue; }
+        unit += g.units;
+        if (g.first >= g.last) continue;                 // (only some of its lead)
         const uint32_t row0 = g.row_tile * R;
-        const AttnRow row = attn_row(a, e, row0 + (lane & 31));
-        AttnAcc<D> acc;
-        attn_clear<D>(acc);
-        uint4_t qf[D / 16];
-        attn_load_q<ActT, D>(a, row, g.kv_head, qf);
+        AttnRow row[RT];
+        float4_t o[RT][MT];
+        float m[RT], l[RT];
+        uint4_t qf[RT][KS];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            row[t] = attn_row(a, e, row0 + 16 * t + col);
+            m[t] = -__builtin_inff();
+            l[t] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < MT; ++j) o[t][j] = float4_t{0, 0, 0, 0};
+            const uint16_t* q = a.q + (size_t)row[t].token * a.q_stride + (size_t)(g.kv_head * a.group + row[t].head) * D + 8 * quarter;
+            attn_load_q<KS>(a, row[t], q, 32, qf[t]);
+        }
 #pragma unroll 1
         for (int run = 0; run < 2; ++run) {
-            const AttnRun u = attn_run(a, e, run, row0, row);
-            const int32_t tile0 = run ? (int32_t)e.front_tiles : 0, tiles = (u.len + 31) / 32;
-            const AttnBounds b = attn_bounds(a, row, run ? (int32_t)e.prefix : 0, u.len);
-            const int32_t* table = run ? a.page_table + (size_t)e.sequence * a.pages_per_sequence : a.prefix_table;
+            const int32_t len = (int32_t)(run ? e.own : e.front), run_base = run ? (int32_t)e.prefix : 0;
+            const int32_t tile0 = run ? (int32_t)e.front_tiles : 0, tiles = (len + 31) / 32;
             int32_t t1 = (int32_t)g.last - tile0, tile = (int32_t)g.first - tile0;
             t1 = t1 > tiles ? tiles : t1;
             // (the segment's tiles are those that one of its rows sees: none in between is to be skipped)
             tile = (tile < 0 ? 0 : tile) + (int32_t)wave;
             if (tile >= t1) continue;
-            // K of the next tile is under way while this one's probabilities and V are worked on, V while the scores are
-            AttnTile<SMALL> at = attn_tile<SMALL, D>(a, table, g.kv_head, (uint32_t)u.len, (uint32_t)tile);
-            uint4_t kf[D / 16];
-            attn_load_k<D, SMALL>(a, at, kf);
+            const int32_t* table = run ? a.page_table + (size_t)e.sequence * a.pages_per_sequence : a.prefix_table;
+            AttnBounds b[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) b[t] = attn_bounds(a, row[t], run_base, len);
+            const AttnRun u = attn_run(a, e, run, row0, R, b, RT);
+            AttnTile at = attn_tile<D>(a, table, g.kv_head, (uint32_t)len, (uint32_t)tile);
+            uint4_t kf[2][KS];
+            auto load_k = [&](const AttnTile& x) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint16_t* k = a.k_cache + x.page[h] + (((quarter << a.page_shift) + x.off[h] + col) << 3);
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) kf[h][s] = *reinterpret_cast<const uint4_t*>(k + ((uint32_t)(4 * s) << (a.page_shift + 3)));
+                }
+            };
+            load_k(at);
 #pragma unroll 1
             for (; tile < t1; tile += 4) {
+                // K of the next tile is under way while this one's probabilities and V are worked on, V while the scores are
                 const int32_t key0 = tile * (int32_t)smelt_serving::kKeyTile;
-                AttnV<D> vf;
-                float16_t s;
-                attn_load_v<D, SMALL>(a, at, vf);
-                const AttnTile<SMALL> next = attn_tile<SMALL, D>(a, table, g.kv_head, (uint32_t)u.len, (uint32_t)(tile + 4 < t1 ? tile + 4 : tile));
-                attn_scores<ActT, D, SMALL>(a, qf, kf, s);
+                uint32_t vf[8][VC][VE / 2];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const uint16_t* v = a.v_cache + at.page[r / 4] + (at.off[r / 4] + 4 * quarter + r % 4) * D + col * VE;
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        if constexpr (VE == 8) { const uint4_t x = *reinterpret_cast<const uint4_t*>(v + 128 * c); vf[r][c][0] = x.x; vf[r][c][1] = x.y; vf[r][c][2] = x.z; vf[r][c][3] = x.w; }
+                        else { const uint2_t x = *reinterpret_cast<const uint2_t*>(v); vf[r][c][0] = x.x; vf[r][c][1] = x.y; }
+                    }
+                }
+                const AttnTile next = attn_tile<D>(a, table, g.kv_head, (uint32_t)len, (uint32_t)(tile + 4 < t1 ? tile + 4 : tile));
+                float4_t s[RT][2];
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        s[t][h] = attn_mfma16<ActT>(kf[h][0], qf[t][0], float4_t{0, 0, 0, 0});
+#pragma unroll
+                        for (int k = 1; k < KS; ++k) s[t][h] = attn_mfma16<ActT>(kf[h][k], qf[t][k], s[t][h]);
+                    }
                 __builtin_amdgcn_sched_barrier(0);
-                attn_load_k<D, SMALL>(a, next, kf);      // (once more the last tile's, from cache, at the end)
+                load_k(next);                            // (once more the last tile's, from cache, at the end)
                 __builtin_amdgcn_sched_barrier(0);
-                const bool bad = at.known != 3u;
-                if (bad || attn_masked(u, key0)) attn_hide(s, key0, b, at.known);
-                attn_softmax<D, 1>(scale, acc, &s);
-                if (bad || key0 + (int32_t)smelt_serving::kKeyTile > u.len) attn_clear_v<D, SMALL>(vf, at, key0, u.len);
-                attn_values<ActT, D>(acc, s, vf);
+                // Values of keys behind the run's end, or on a page that is none of the pool's, are whatever memory holds: zero them, since
+                // a zero probability does not silence an infinity or a NaN.
+                if (at.known != 3u || key0 + (int32_t)smelt_serving::kKeyTile > len) {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const bool ok = key0 + 16 * (r / 4) + 4 * (int32_t)quarter + r % 4 < len && ((at.known >> (r / 4)) & 1u);
+#pragma unroll
+                        for (int c = 0; c < VC; ++c)
+#pragma unroll
+                            for (int k = 0; k < VE / 2; ++k) vf[r][c][k] = ok ? vf[r][c][k] : 0u;
+                    }
+                }
+                const bool edge = at.known != 3u || attn_masked(u, key0);
+                uint4_t pf[RT];
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    if (edge) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int32_t key = key0 + 16 * h + 4 * (int32_t)quarter + i;
+                                const bool ok = key >= b[t].lo && key < b[t].hi && ((at.known >> h) & 1u);
+                                s[t][h][i] = ok ? s[t][h][i] : -__builtin_inff();
+                            }
+                    }
+                    float top = __builtin_fmaxf(s[t][0][0], s[t][1][0]);
+#pragma unroll
+                    for (int i = 1; i < 4; ++i) top = __builtin_fmaxf(__builtin_fmaxf(top, s[t][0][i]), s[t][1][i]);
+                    top = attn_quarters_max(top);
+                    if (__any(top > m[t] + scale.slack)) {      // also the first finite score: the maximum starts at -inf
+                        const float to = __builtin_fmaxf(m[t], top);
+                        const float f = to == -__builtin_inff() ? 1.0f : attn_exp2((m[t] - to) * scale.c);
+                        l[t] *= f;
+#pragma unroll
+                        for (int j = 0; j < MT; ++j) o[t][j] *= f;
+                        m[t] = to;
+                    }
+                    const float shift = m[t] == -__builtin_inff() ? 0.0f : -m[t] * scale.c;
+                    float p[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) p[i] = attn_exp2(__builtin_fmaf(s[t][i / 4][i % 4], scale.c, shift));
+                    l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                    pf[t] = uint4_t{attn_pack2<ActT>(p[0], p[1]), attn_pack2<ActT>(p[2], p[3]), attn_pack2<ActT>(p[4], p[5]), attn_pack2<ActT>(p[6], p[7])};
+                }
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    const int c = j / VE, x = (j % VE) / 2;
+                    const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+                    uint4_t v;
+                    v.x = __builtin_amdgcn_perm(vf[1][c][x], vf[0][c][x], sel);
+                    v.y = __builtin_amdgcn_perm(vf[3][c][x], vf[2][c][x], sel);
+                    v.z = __builtin_amdgcn_perm(vf[5][c][x], vf[4][c][x], sel);
+                    v.w = __builtin_amdgcn_perm(vf[7][c][x], vf[6][c][x], sel);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) o[t][j] = attn_mfma16<ActT>(v, pf[t], o[t][j]);
+                }
                 at = next;
             }
         }
-        // the waves meet
-        const float l = attn_halves_sum(acc.l);
-        const uint32_t half = lane >> 5;
-        if (lane < 32) { sh.m[wave][lane] = acc.m; sh.l[wave][lane] = l; }
-        if (row.live) {
-            constexpr int E = D / 32;
+        // the waves meet: o[t][j][i] is value VE (4 quarter + i) + j % VE + 128 (j / VE) of the lane's row
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float* dst = &sh.o[wave][lane & 31][E * (8 * (i / 4) + 4 * half + i % 4)];
-                if constexpr (E >= 4) {
+        for (int t = 0; t < RT; ++t) {
+            const float sum = attn_quarters_sum(l[t]);
+            if (lane < 16) { sh.m[wave][16 * t + lane] = m[t]; sh.l[wave][16 * t + lane] = sum; }
+            if (row[t].live) {
 #pragma unroll
-                    for (int j = 0; j < E; j += 4) *reinterpret_cast<float4_t*>(dst + j) = float4_t{acc.o[j][i], acc.o[j + 1][i], acc.o[j + 2][i], acc.o[j + 3][i]};
-                } else {
+                for (int c = 0; c < VC; ++c)
 #pragma unroll
-                    for (int j = 0; j < E; ++j) dst[j] = acc.o[j][i];
-                }
+                    for (int i = 0; i < 4; ++i) {
+                        float* dst = &sh.o[wave][16 * t + col][VE * (4 * quarter + i) + 128 * c];
+#pragma unroll
+                        for (int j = 0; j < VE; j += 4)
+                            *reinterpret_cast<float4_t*>(dst + j) = float4_t{o[t][c * VE + j][i], o[t][c * VE + j + 1][i], o[t][c * VE + j + 2][i], o[t][c * VE + j + 3][i]};
+                    }
             }
         }
         __syncthreads();
@@ -537,61 +573,69 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
 #pragma unroll 1
         for (uint32_t item = threadIdx.x; item < rows_live * (D / 4); item += blockDim.x) {
             const uint32_t r = item / (D / 4), d = (item % (D / 4)) * 4;
-            float m = sh.m[0][r];
+            float top = sh.m[0][r];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) m = __builtin_fmaxf(m, sh.m[w][r]);
+            for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, sh.m[w][r]);
             float4_t y = {0, 0, 0, 0};
             float sum = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = m == -__builtin_inff() ? 1.0f : attn_exp2((sh.m[w][r] - m) * scale.c);
+                const float f = top == -__builtin_inff() ? 1.0f : attn_exp2((sh.m[w][r] - top) * scale.c);
                 y += f * *reinterpret_cast<const float4_t*>(&sh.o[w][r][d]);
                 sum += f * sh.l[w][r];
             }
             const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
             if (!g.whole) {
                 *reinterpret_cast<float4_t*>(piece + 2 * R + r * D + d) = y;
-                if (d == 0) { piece[r] = m; piece[R + r] = sum; }
+                if (d == 0) { piece[r] = top; piece[R + r] = sum; }
             } else if (a.part != smelt_serving::kWholeSequences) {
                 float* dst = attn_whole_row(a, token, head, D);
                 *reinterpret_cast<float4_t*>(dst + d) = y;
-                if (d == 0) { dst[D] = m; dst[D + 1] = sum; }
+                if (d == 0) { dst[D] = top; dst[D + 1] = sum; }
             } else {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 *reinterpret_cast<uint2_t*>(a.out + ((size_t)token * a.heads + head) * D + d) = uint2_t{attn_pack2<ActT>(y.x * inv, y.y * inv), attn_pack2<ActT>(y.z * inv, y.w * inv)};
             }
         }
         __syncthreads();
-        unit += g.last - g.first;
     }
 }
 
 // Many rows (prompts, the prefix against a batch): bound by the matrix cores.  A workgroup's WAVES waves hold 32 rows each and walk
-// the key tiles together: a stage of NS tiles is read once from the cache into registers while the stage before it is
-// worked on, and put down in LDS (two stages, one barrier a stage), from where every wave takes it: K in operand order, V through the
-// transposing LDS read (16 lanes take 4 keys x 16 values and get one value of 4 keys each), its 16-byte pieces placed so that the
-// four keys of such a read lie on different banks.  Heads of up to 128 run two waves a SIMD, one's softmax under the other's
-// products; heads of 256 need the whole register file for one.
+// the key tiles together, in stages of NS tiles that are loaded from the cache straight to LDS (no registers in between) while the
+// BUFFERS - 1 stages before are waited for and worked on, one barrier a stage.  Every wave takes its operands from there: K in
+// operand order, V through the transposing LDS read (16 lanes take 4 keys x 16 values and get one value of 4 keys each), the
+// 16-byte pieces of V rows placed so that the four keys of such a read lie on different banks.
 typedef short attn_short4_t __attribute__((ext_vector_type(4)));
+constexpr int kAttnBuffers = 4;
 template <int D, int NS>
-struct AttnTilesShared { uint16_t k[2][NS][32 * D], v[2][NS][32 * D]; };
+struct AttnTilesShared { uint16_t tile[kAttnBuffers][NS][2][32 * D]; };      // K, V
 
-// where 16-byte piece c of V row r lies in its row: bits 2 and 3 of the piece turned by the row
+// 16-byte piece c of V row r lies at piece c ^ (4 * turn): of rows 4 apart in a read, on different banks
 template <int D>
 __device__ __forceinline__ uint32_t attn_v_turn(uint32_t row) { return D == 64 ? (row >> 1) & 1u : row & 3u; }
 
-template <class ActT, int D, int WAVES, int NS, bool SMALL>
+// 16 bytes a lane from `src` to LDS at `lds` + 16 * lane; counts as a vector load, in order
+__device__ __forceinline__ void attn_load_lds(const uint16_t* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+}
+// waits until at most N of the wave's vector loads are under way
+template <int N>
+__device__ __forceinline__ void attn_wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+
+template <class ActT, int D, int WAVES, int NS>
 __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     AttnTilesShared<D, NS>& sh = *reinterpret_cast<AttnTilesShared<D, NS>*>(smem);
     constexpr uint32_t R = 32 * WAVES, T = 64 * WAVES;
-    constexpr int P = 8 * D / T;                         // 16-byte pieces of a key tile (K, then V) that a thread stages
+    constexpr int P = 8 * D / T;                         // 16-byte pieces of a key tile (K, then V) that a thread loads
     const AttnWork work = find_work<kFirstUnit>(a, blockIdx.x);
     if (work.entry == ~0u) return;
     uint32_t unit = work.at, index = work.entry, base = work.base;
     const uint32_t unit_end = work.split.whole ? unit + 1 : smelt_serving::attention_start(work.split, blockIdx.x + 1);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, half = lane >> 5;
     const AttnScale scale = attn_scale(a);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem);
     // the lane's share of a transposing read: key row and 8-byte piece; the pieces of 32 values further on are turned by the row
     const uint32_t v_row = 4 * half + (lane & 15) / 4, v_turn = attn_v_turn<D>(v_row);
     const uint32_t v_lane = v_row * 2 * D + ((lane & 31) / 16) * 32 + (lane & 3) * 8;
@@ -601,118 +645,122 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
         AttnSegment g;
         if (work.split.whole) attn_whole_segment(a, e, unit - base, g);
         else if (!attn_segment(a, e, base, unit, unit_end, g)) { base = g.begin; ++index; continue; }
+        unit += g.units;
+        if (g.first >= g.last) continue;                 // (only some of its lead)
+        const int32_t* own_table = a.page_table + (size_t)(e.sequence < 0 ? 0 : e.sequence) * a.pages_per_sequence;
+
+        uint32_t pages_known = 0;                         // four bits a buffer, two a tile: the tile's halves are on pages of the pool's
+        auto fetch = [&](uint32_t first, uint32_t buffer) {
+            pages_known &= ~(15u << (4 * buffer));
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                // (past the part's end: its last tile once more, so that every stage is the same number of loads)
+                uint32_t ct = first + n < g.last ? first + n : g.last - 1;
+                if (ct >= e.tiles) continue;             // (no keys at all)
+                const bool run = ct >= e.front_tiles;
+                const uint32_t tile = ct - (run ? e.front_tiles : 0u);
+                const AttnTile at = attn_tile<D>(a, run ? own_table : a.prefix_table, g.kv_head, run ? e.own : e.front, tile);
+                pages_known |= at.known << (4 * buffer + 2 * n);
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const uint32_t piece = p * T + threadIdx.x;
+                    const uint32_t lds = lds0 + (((buffer * NS + n) * 2) * 32 * D * 2) + (p * T + wave * 64) * 16;
+                    const uint16_t* src;
+                    if ((p * T + wave * 64) < 4 * D) {                                                       // K: [dim / 8][key][8]
+                        const uint32_t chunk = piece / 32, key = piece % 32;
+                        src = a.k_cache + (key < 16 ? at.page[0] : at.page[1]) + (((chunk << a.page_shift) + (key < 16 ? at.off[0] : at.off[1]) + (key & 15)) << 3);
+                    } else {                                                                                 // V: [key][dim]
+                        const uint32_t key = (piece - 4 * D) / (D / 8), col = ((piece - 4 * D) % (D / 8)) ^ (4 * attn_v_turn<D>(key));
+                        src = a.v_cache + (key < 16 ? at.page[0] : at.page[1]) + ((key < 16 ? at.off[0] : at.off[1]) + (key & 15)) * D + col * 8;
+                    }
+                    attn_load_lds(src, __builtin_amdgcn_readfirstlane(lds));
+                }
+            }
+        };
+        const uint32_t stages = (g.last - g.first + NS - 1) / NS;
+#pragma unroll 1
+        for (uint32_t s = 0; s < kAttnBuffers - 1 && s < stages; ++s) fetch(g.first + s * NS, s);
+
         const uint32_t row0 = g.row_tile * R + wave * 32;
         const AttnRow row = attn_row(a, e, row0 + (lane & 31));
         AttnAcc<D> acc;
         attn_clear<D>(acc);
         uint4_t qf[D / 16];
-        attn_load_q<ActT, D>(a, row, g.kv_head, qf);
-        const AttnRun front = attn_run(a, e, 0, row0, row), own = attn_run(a, e, 1, row0, row);
-        const AttnBounds front_b = attn_bounds(a, row, 0, front.len), own_b = attn_bounds(a, row, (int32_t)e.prefix, own.len);
-        const int32_t* own_table = a.page_table + (size_t)(e.sequence < 0 ? 0 : e.sequence) * a.pages_per_sequence;
+        attn_load_q<D / 16>(a, row, a.q + (size_t)row.token * a.q_stride + (size_t)(g.kv_head * a.group + row.head) * D + 8 * half, 16, qf);
+        const AttnBounds front_b = attn_bounds(a, row, 0, (int32_t)e.front), own_b = attn_bounds(a, row, (int32_t)e.prefix, (int32_t)e.own);
+        const AttnRun front = attn_run(a, e, 0, row0, 32, &front_b, 1), own = attn_run(a, e, 1, row0, 32, &own_b, 1);
+        attn_wait_loads<0>();                             // (the compiler counts q's loads alone: from here on only stages are under way)
 
-        uint4_t stage[NS][P];
-        uint32_t known_next = 0;                          // two bits a tile: its pages are the pool's
-        auto fetch = [&](uint32_t first) {
-            known_next = 0;
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const uint32_t ct = first + n;
-                const bool some = ct < g.last && ct < e.tiles, run = ct >= e.front_tiles;
-                if (!some) {
-#pragma unroll
-                    for (int p = 0; p < P; ++p) stage[n][p] = uint4_t{0, 0, 0, 0};
-                    continue;
-                }
-                const uint32_t tile = ct - (run ? e.front_tiles : 0u), len = run ? e.own : e.front;
-                const AttnTile<SMALL> at = attn_tile<SMALL, D>(a, run ? own_table : a.prefix_table, g.kv_head, len, tile);
-                known_next |= at.known << (2 * n);
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const uint32_t piece = p * T + threadIdx.x;
-                    if (piece < 4 * D) {                                                                    // K: [dim / 8][key][8]
-                        const uint32_t chunk = piece / 32, key = piece % 32;
-                        const size_t kb = SMALL && key >= 16 ? at.base[SMALL ? 1 : 0] : at.base[0];
-                        stage[n][p] = *reinterpret_cast<const uint4_t*>(a.k_cache + kb + (((chunk << a.page_shift) + (SMALL ? key & 15 : at.off + key)) << 3));
-                    } else {                                                                                // V: [key][dim]
-                        const uint32_t key = (piece - 4 * D) / (D / 8), col = (piece - 4 * D) % (D / 8);
-                        const size_t vb = SMALL && key >= 16 ? at.base[SMALL ? 1 : 0] : at.base[0];
-                        const uint4_t v = *reinterpret_cast<const uint4_t*>(a.v_cache + vb + (SMALL ? key & 15 : at.off + key) * D + col * 8);
-                        // (values behind the run's end or outside the pool are whatever memory holds)
-                        const bool ok = tile * 32 + key < len && ((at.known >> (key / 16)) & 1u);
-                        stage[n][p] = ok ? v : uint4_t{0, 0, 0, 0};
-                    }
-                }
-            }
-        };
-        auto put = [&](int buffer) {
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const uint32_t piece = p * T + threadIdx.x;
-                    if (piece < 4 * D) reinterpret_cast<uint4_t*>(sh.k[buffer][n])[piece] = stage[n][p];
-                    else {
-                        const uint32_t key = (piece - 4 * D) / (D / 8), col = (piece - 4 * D) % (D / 8);
-                        reinterpret_cast<uint4_t*>(sh.v[buffer][n])[key * (D / 8) + (col ^ (4 * attn_v_turn<D>(key)))] = stage[n][p];
-                    }
-                }
-        };
-        fetch(g.first);
-        put(0);
-        uint32_t known = known_next;
-        __syncthreads();
-        int buffer = 0;
 #pragma unroll 1
-        for (uint32_t first = g.first; first < g.last; first += NS, buffer ^= 1) {
-            const bool more = first + NS < g.last;
-            if (more) fetch(first + NS);
-            // what the wave's rows see of the stage
-            bool seen = false, edge[NS];
+        for (uint32_t stage = 0; stage < stages; ++stage) {
+            const uint32_t first = g.first + stage * NS, buffer = stage % kAttnBuffers;
+            // this stage is complete when only the later ones' loads are left
+            if (stage + kAttnBuffers - 1 <= stages) attn_wait_loads<(kAttnBuffers - 2) * P * NS>();
+            else attn_wait_loads<0>();
+            __syncthreads();
+            const uint32_t stage_known = pages_known >> (4 * buffer);
+            if (stage + kAttnBuffers - 1 < stages) fetch(first + (kAttnBuffers - 1) * NS, (stage + kAttnBuffers - 1) % kAttnBuffers);
+            // what the wave's rows see of the stage, and what there is of it (a tile past the part's end: nothing)
+            bool seen = false, edge[NS], ragged = false;
+            uint32_t known[NS];
             int32_t key0[NS];
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
                 const uint32_t ct = first + n;
                 const bool some = ct < g.last && ct < e.tiles, run = ct >= e.front_tiles;
                 const AttnRun& u = run ? own : front;
-                key0[n] = (int32_t)(ct - (run ? e.front_tiles : 0u)) * (int32_t)smelt_serving::kKeyTile;
+                const uint32_t tile = ct - (run ? e.front_tiles : 0u), len = run ? e.own : e.front;
+                key0[n] = (int32_t)tile * (int32_t)smelt_serving::kKeyTile;
+                known[n] = some ? (stage_known >> (2 * n)) & 3u : 0u;
                 seen = seen || (some && attn_seen(u, key0[n]));
-                edge[n] = !some || ((known >> (2 * n)) & 3u) != 3u || attn_masked(u, key0[n]);
+                edge[n] = known[n] != 3u || attn_masked(u, key0[n]);
+                ragged = ragged || known[n] != 3u || tile * 32 + 32 > len;
             }
-            if (seen) {
-                float16_t s[NS];
-#pragma unroll
+            if (ragged) {
+                // Values of keys behind the run's end, or on a page that is none of the pool's, are whatever memory holds: zero them, since a
+                // zero probability does not silence an infinity or a NaN.
+#pragma unroll 1
                 for (int n = 0; n < NS; ++n) {
-                    const uint4_t* kl = reinterpret_cast<const uint4_t*>(sh.k[buffer][n]) + lane;
-                    s[n] = attn_mfma<ActT>(kl[0], qf[0], float16_t{});
-#pragma unroll
-                    for (int d = 1; d < D / 16; ++d) s[n] = attn_mfma<ActT>(kl[d * 64], qf[d], s[n]);
+                    const uint32_t len = first + n >= e.front_tiles ? e.own : e.front;
+                    uint4_t* v = reinterpret_cast<uint4_t*>(sh.tile[buffer][n][1]);
+                    for (uint32_t p = threadIdx.x; p < 4 * D; p += T) {
+                        const uint32_t key = p / (D / 8);
+                        if ((uint32_t)key0[n] + key >= len || !((known[n] >> (key / 16)) & 1u)) v[p] = uint4_t{0, 0, 0, 0};
+                    }
                 }
+                __syncthreads();
+            }
+            if (!seen) continue;
+            float16_t s[NS];
 #pragma unroll
-                for (int n = 0; n < NS; ++n)
-                    if (edge[n]) attn_hide(s[n], key0[n], first + n >= e.front_tiles ? own_b : front_b, first + n < g.last && first + n < e.tiles ? known >> (2 * n) : 0u);
-                attn_softmax<D, NS>(scale, acc, s);
+            for (int n = 0; n < NS; ++n) {
+                const uint4_t* kl = reinterpret_cast<const uint4_t*>(sh.tile[buffer][n][0]) + lane;
+                s[n] = attn_mfma<ActT>(kl[0], qf[0], float16_t{});
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    const char* vl = reinterpret_cast<const char*>(sh.v[buffer][n]) + v_lane;
+                for (int d = 1; d < D / 16; ++d) s[n] = attn_mfma<ActT>(kl[d * 64], qf[d], s[n]);
+            }
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint4_t pf = attn_pack<ActT>(s[n], u);
+            for (int n = 0; n < NS; ++n)
+                if (edge[n]) attn_hide(s[n], key0[n], first + n >= e.front_tiles ? own_b : front_b, known[n]);
+            attn_softmax<D, NS>(scale, acc, s);
 #pragma unroll
-                        for (int j = 0; j < D / 32; ++j) {
-                            const char* at = vl + 16 * u * 2 * D + ((j & ~3) | ((j & 3) ^ v_turn)) * 64;
-                            typedef __attribute__((address_space(3))) attn_short4_t* lds_ptr;
-                            const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at));
-                            const uint2_t hi = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 8 * 2 * D)));
-                            acc.o[j] = attn_mfma<ActT>(uint4_t{lo.x, lo.y, hi.x, hi.y}, pf, acc.o[j]);
-                        }
+            for (int n = 0; n < NS; ++n) {
+                const char* vl = reinterpret_cast<const char*>(sh.tile[buffer][n][1]) + v_lane;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint4_t pf = attn_pack<ActT>(s[n], u);
+#pragma unroll
+                    for (int j = 0; j < D / 32; ++j) {
+                        const char* at = vl + 16 * u * 2 * D + ((j & ~3) | ((j & 3) ^ v_turn)) * 64;
+                        typedef __attribute__((address_space(3))) attn_short4_t* lds_ptr;
+                        const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at));
+                        const uint2_t hi = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 8 * 2 * D)));
+                        acc.o[j] = attn_mfma<ActT>(uint4_t{lo.x, lo.y, hi.x, hi.y}, pf, acc.o[j]);
                     }
                 }
             }
-            if (more) put(buffer ^ 1);
-            known = known_next;
-            __syncthreads();
         }
+        __syncthreads();                                  // (the next part's loads overwrite the stages)
         // a lane holds its row's values 32 j + 8 (i / 4) + 4 half + i % 4
         float* piece = a.pieces + ((size_t)blockIdx.x * 2 + (g.first == g.tiles.lo ? 1 : 0)) * smelt_serving::piece_floats(R, D);
         const float l = attn_halves_sum(acc.l);
@@ -740,7 +788,6 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                         *reinterpret_cast<float4_t*>(dst + 4 * half + 32 * j + 2 * i) = float4_t{acc.o[j][i], acc.o[j][i + 1], acc.o[j][i + 2], acc.o[j][i + 3]};
             }
         }
-        unit += work.split.whole ? 1 : g.last - g.first;
     }
 }
 
@@ -792,7 +839,7 @@ __device__ __forceinline__ void attn_combine(const AttentionArgs& a) {
     AttnSegment g;
     if (!attn_segment(a, e, work.base, work.at, ~0u, g)) return;
     const uint32_t end = g.begin + (g.tiles.hi - g.tiles.lo);
-    if (g.begin == work.at || smelt_serving::attention_start(work.split, blockIdx.x) > g.begin) return;     // not inside a segment, or not the first
+    if (work.at <= g.begin || smelt_serving::attention_start(work.split, blockIdx.x) > g.begin) return;     // not inside a segment, or not the first
     const uint32_t w1 = smelt_serving::attention_owner(work.split, end - 1);
     const uint32_t row0 = g.row_tile * a.row_tile, left = e.tokens * a.group - row0, rows = left < a.row_tile ? left : a.row_tile;
 #pragma unroll 1
@@ -828,8 +875,8 @@ __device__ __forceinline__ void attn_combine_shared(const smelt_serving::Attenti
             uint32_t begin = w.base;
             AttentionTiles s = smelt_serving::attention_tiles(x, e, 0);
 #pragma unroll 1
-            for (uint32_t t = 1; t <= row_tile; ++t) { begin += (s.hi - s.lo) * x.kv_heads; s = smelt_serving::attention_tiles(x, e, t); }
-            begin += (s.hi - s.lo) * kv_head;
+            for (uint32_t t = 1; t <= row_tile; ++t) { begin += (s.hi - s.lo + x.lead) * x.kv_heads; s = smelt_serving::attention_tiles(x, e, t); }
+            begin += (s.hi - s.lo + x.lead) * kv_head + x.lead;
             uint32_t w0 = 0, w1 = 0;
             if (!w.split.whole) { w0 = smelt_serving::attention_owner(w.split, begin); w1 = smelt_serving::attention_owner(w.split, begin + (s.hi - s.lo) - 1); }
             if (w0 == w1) {
@@ -846,10 +893,9 @@ __device__ __forceinline__ void attn_combine_shared(const smelt_serving::Attenti
 }  // namespace smelt
 
 // (one wave a SIMD where accumulators, q and the tiles in flight take the whole register file)
-#define SMELT_ATTENTION_KERNELS(T, ACT, D, STREAM_WAVES, WAVES, NS, TILE_WAVES)                                                                                                   \
-    extern "C" __global__ __launch_bounds__(256, STREAM_WAVES) void smelt_attention_stream_d##D##_##T(smelt_serving::AttentionArgs a) { smelt::attn_stream<ACT, D, false>(a); }          \
-    extern "C" __global__ __launch_bounds__(256, STREAM_WAVES) void smelt_attention_stream_d##D##_p16_##T(smelt_serving::AttentionArgs a) { smelt::attn_stream<ACT, D, true>(a); }       \
-    extern "C" __global__ __launch_bounds__(64 * WAVES, TILE_WAVES) void smelt_attention_tiles_d##D##_##T(smelt_serving::AttentionArgs a) { smelt::attn_tiles<ACT, D, WAVES, NS, false>(a); }   \
-    extern "C" __global__ __launch_bounds__(64 * WAVES, TILE_WAVES) void smelt_attention_tiles_d##D##_p16_##T(smelt_serving::AttentionArgs a) { smelt::attn_tiles<ACT, D, WAVES, NS, true>(a); } \
-    extern "C" __global__ __launch_bounds__(256) void smelt_attention_join_d##D##_##T(smelt_serving::AttentionArgs a) { smelt::attn_combine<ACT, D>(a); }                              \
-    extern "C" __global__ __launch_bounds__(256) void smelt_attention_join_shared_d##D##_##T(smelt_serving::AttentionJoinArgs a) { smelt::attn_combine_shared<ACT, D>(a); }
+#define SMELT_ATTENTION_KERNELS(T, ACT, D, STREAM16, STREAM32, WAVES, NS, TILE_WAVES)                                                                                           \
+    extern "C" __global__ __launch_bounds__(256, STREAM16) void smelt_attention_stream16_d##D##_##T(smelt_serving::AttentionArgs a) { smelt::attn_stream<ACT, D, 1>(a); }             \
+    extern "C" __global__ __launch_bounds__(256, STREAM32) void smelt_attention_stream32_d##D##_##T(smelt_serving::AttentionArgs a) { smelt::attn_stream<ACT, D, 2>(a); }             \
+    extern "C" __global__ __launch_bounds__(64 * WAVES, TILE_WAVES) void smelt_attention_tiles_d##D##_##T(smelt_serving::AttentionArgs a) { smelt::attn_tiles<ACT, D, WAVES, NS>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void smelt_attention_join_d##D##_##T(smelt_serving::AttentionArgs a) { smelt::attn_combine<ACT, D>(a); }                            \
+    extern "C" __global__ __launch_bounds__(1024) void smelt_attention_join_shared_d##D##_##T(smelt_serving::AttentionJoinArgs a) { smelt::attn_combine_shared<ACT, D>(a); }

@@ -43,8 +43,9 @@ struct RopeArgs {
 // pages of its row of the page table; keys 0 .. prefix_len of every sequence are the shared prefix.  A launch covers a list of
 // work entries: the sequences with their prefix and own keys, the sequences with their own keys only, or the prefix against all rows at
 // once.  An entry is cut into segments: a tile of `row_tile` rows (token, head of the group) of one kv head, against the key
-// tiles that any of its rows sees.  The workgroups take equal runs of the resulting units (one unit: one key tile of one
-// segment, row tiles ascending, within them the kv heads, within them the key tiles), or a segment each where there are enough of those.
+// tiles that any of its rows sees.  The workgroups take equal runs of the resulting units: `lead` units for beginning a segment,
+// then one for each of its key tiles; row tiles ascending, within them the kv heads, within them the units.  Where there are enough
+// segments for that, each workgroup takes one.
 constexpr uint32_t kKeyTile = 32;
 enum AttentionPart : uint32_t { kWholeSequences = 0, kOwnKeys = 1, kPrefix = 2 };
 
@@ -64,6 +65,7 @@ struct AttentionArgs {
     uint32_t pages = 0, page_shift = 0, pages_per_sequence = 0, prefix_pages = 0;
     uint32_t window = 0, q_stride = 0, workgroups = 0, part = 0;
     uint32_t row_tile = 0;
+    uint32_t lead = 0;             // what beginning a segment costs, in key tiles
     uint32_t least_units = 1;      // a workgroup takes at least this many units
     uint32_t whole_from = ~0u;     // segments from which on each workgroup takes one
     float scale_log2 = 0;          // |scale| * log2(e)
@@ -142,7 +144,7 @@ SMELT_HD AttentionTiles attention_tiles(const AttentionArgs& a, const AttentionE
 SMELT_HD uint32_t attention_units(const AttentionArgs& a, const AttentionEntry& e) {
     uint32_t n = 0;
 #pragma unroll 1
-    for (uint32_t r = 0; r < e.row_tiles; ++r) { const AttentionTiles t = attention_tiles(a, e, r); n += t.hi - t.lo; }
+    for (uint32_t r = 0; r < e.row_tiles; ++r) { const AttentionTiles t = attention_tiles(a, e, r); n += t.hi - t.lo + a.lead; }
     return n * a.kv_heads;
 }
 SMELT_HD uint32_t attention_segments(const AttentionArgs& a, const AttentionEntry& e) { return a.kv_heads * e.row_tiles; }

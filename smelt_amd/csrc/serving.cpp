@@ -13,7 +13,7 @@ using namespace smelt_serving;
 
 namespace {
 
-constexpr uint32_t kStreamRows = 32;     // row tile of the streaming attention kernel
+constexpr uint32_t kSegmentLead = 4;     // what beginning a segment of rows and keys costs, in key tiles
 
 // "_d256" at `at`: the number behind the letters, and the position behind it
 bool number_after(const std::string& s, const char* letters, size_t* at, uint32_t* out) {
@@ -82,10 +82,8 @@ ResolveStatus resolve_serving(const std::string& entry, const char* act, Resolve
         out->family = shared ? kFamPagedAttentionShared : kFamPagedAttention;
         out->kinds = shared ? "PPPPPPPPPUUUUUFUUUUUU" : "PPPPPPPUUUUFUUUUUU";
         out->appended = {dim, heads, kv_heads, page};
-        const std::string d = "d" + std::to_string(dim);
-        const std::string small = page == 16 ? "_p16" : "";
-        out->serving_symbols = {"smelt_attention_stream_" + d + small + t, "smelt_attention_tiles_" + d + small + t, "smelt_attention_join_" + d + t,
-                                "smelt_attention_join_shared_" + d + t};
+        const std::string tail = "_d" + std::to_string(dim) + t;
+        for (const char* k : {"stream16", "stream32", "tiles", "join", "join_shared"}) out->serving_symbols.push_back(std::string("smelt_attention_") + k + tail);
         out->symbol = out->serving_symbols[0];
         return kResolveOk;
     }
@@ -278,64 +276,67 @@ int Planner::attention() {
     a.out = P<uint16_t>(6);
     if (shared && a.prefix_pages) { a.prefix_table = P<int32_t>(7); a.prefix_len = P<int32_t>(8); }
 
-    // The streaming kernel takes the sequences while they have few rows each (one row tile on average), the prefix then being read once
-    // against all rows; the tile kernel takes longer runs of rows, whose tiles read prefix and own keys alike.
+    // The streaming kernel takes the sequences while they have few rows each (one tile of 16 or 32 rows on average), the prefix then
+    // being read once against all rows; the tile kernel takes longer runs of rows, whose tiles read prefix and own keys alike.
     const uint64_t rows = (uint64_t)a.tokens * a.group;
-    const bool stream = rows <= (uint64_t)kStreamRows * a.sequences;
+    const bool stream = rows <= (uint64_t)32 * a.sequences;
     const uint32_t tile_rows = dim == 256 ? 128 : 256;
+    auto row_tile = [&](uint64_t of, uint64_t over) { return of <= 16 * over ? 16u : (of <= 32 * over ? 32u : tile_rows); };
     // The parts of cut segments live in the context's workspace: two a workgroup; with the prefix apart, so do the rows
     // of segments that one workgroup finished.
-    auto slot_bytes = [&](uint32_t row_tile) { return (size_t)piece_floats(row_tile, dim) * 4 * 2; };
+    auto slot_bytes = [&](uint32_t r) { return (size_t)piece_floats(r, dim) * 4 * 2; };
     const size_t row_region = (size_t)a.tokens * a.heads * (dim + 4) * 4;
     char* ws = static_cast<char*>(dev.workspace);
-    auto lay_out = [&](AttentionArgs& x, bool streams, size_t room) {
-        x.row_tile = streams ? kStreamRows : tile_rows;
-        x.least_units = streams ? 4 : 8;       // a key tile for each of four waves; two stages
-        const uint32_t resident = dev.compute_units * (streams && dim != 256 ? 2u : 1u);
-        x.workgroups = (uint32_t)std::min<size_t>(resident, room / slot_bytes(x.row_tile));
+    auto lay_out = [&](AttentionArgs& x, uint32_t r, size_t room) {
+        x.row_tile = r;
+        x.lead = kSegmentLead;
+        x.least_units = x.lead + (r <= 32 ? 4 : 8);       // a key tile for each of four waves; stages to keep under way
+        // workgroups that the register file holds
+        const uint32_t per_cu = r == 16 ? (dim == 256 ? 2 : (dim == 128 ? 3 : 4)) : (r == 32 && dim != 256 ? 2 : 1);
+        x.workgroups = (uint32_t)std::min<size_t>((size_t)dev.compute_units * per_cu, room / slot_bytes(r));
         // a segment each from three quarters of the workgroups on: no parts to write and join
-        x.whole_from = streams ? ~0u : std::max(1u, dev.compute_units * 3 / 4);
+        x.whole_from = r <= 32 ? ~0u : std::max(1u, dev.compute_units * 3 / 4);
     };
-    auto main_step = [&](const AttentionArgs& x, bool streams) {
-        const size_t lds = streams ? (size_t)4 * 32 * (dim + 4) * 4 + 2 * 4 * 32 * 4 : (size_t)2 * 2 * (dim == 256 ? 1 : 2) * 32 * dim * 2;
-        uint32_t grid = x.workgroups;
-        if (!streams) {      // as many as there can be segments
-            const uint64_t entry_rows = (uint64_t)x.tokens * x.group, most = ((entry_rows + x.row_tile - 1) / x.row_tile + (x.part == kPrefix ? 0 : x.sequences)) * x.kv_heads;
-            grid = (uint32_t)std::max<uint64_t>(grid, std::min<uint64_t>(most, 0x7FFFFFFFull));
+    auto main_step = [&](const AttentionArgs& x) {
+        const uint32_t r = x.row_tile;
+        if (r <= 32) {
+            step(r == 16 ? 0 : 1, x, x.workgroups, 1, 1, 256, (size_t)4 * r * (dim + 4) * 4 + 2 * 4 * r * 4);
+            return;
         }
-        step(streams ? 0 : 1, x, grid, 1, 1, streams || dim == 256 ? 256 : 512, lds);
+        // as many as there can be segments
+        const uint64_t most = (((uint64_t)x.tokens * x.group + r - 1) / r + (x.part == kPrefix ? 0 : x.sequences)) * x.kv_heads;
+        step(2, x, (uint32_t)std::max<uint64_t>(x.workgroups, std::min<uint64_t>(most, 0x7FFFFFFFull)), 1, 1, dim == 256 ? 256 : 512, (size_t)4 * (dim == 256 ? 1 : 2) * 2 * 32 * dim * 2);
     };
     // units are counted in 32 bits
     const uint64_t key_tiles = ((uint64_t)a.pages_per_sequence + a.prefix_pages) * page / kKeyTile + 2;
-    const uint64_t row_tiles = rows / (stream ? kStreamRows : tile_rows) + a.sequences + 1;
-    if (row_tiles * a.kv_heads > 0x7FFFFFFFull / key_tiles) return bad("rows times keys pass 2^31 key tiles");
-    const bool prefix = shared && a.prefix_pages;
-    if (stream && prefix && 2 * row_region + slot_bytes(kStreamRows) + slot_bytes(tile_rows) <= dev.workspace_bytes) {
-        const bool front_streams = rows <= kStreamRows;
+    const uint64_t row_tiles = rows / 16 + a.sequences + 1;
+    if (row_tiles * a.kv_heads > 0x7FFFFFFFull / (key_tiles + kSegmentLead)) return bad("rows times keys pass 2^31 key tiles");
+    const uint32_t own_rows = row_tile(rows, a.sequences), front_rows = row_tile(rows, 1);
+    if (stream && shared && a.prefix_pages && 2 * row_region + slot_bytes(own_rows) + slot_bytes(front_rows) <= dev.workspace_bytes) {
         AttentionJoinArgs both;
         both.front = a; both.own = a;
         both.front.part = kPrefix; both.own.part = kOwnKeys;
         both.front.rows = reinterpret_cast<float*>(ws);
         both.own.rows = reinterpret_cast<float*>(ws + row_region);
         const size_t room = dev.workspace_bytes - 2 * row_region;
-        lay_out(both.own, true, room / 2);
-        const size_t own_bytes = (size_t)both.own.workgroups * slot_bytes(kStreamRows);
-        lay_out(both.front, front_streams, room - own_bytes);
+        lay_out(both.own, own_rows, room / 2);
+        const size_t own_bytes = (size_t)both.own.workgroups * slot_bytes(own_rows);
+        lay_out(both.front, front_rows, room - own_bytes);
         if (both.own.workgroups && both.front.workgroups) {
             both.own.pieces = reinterpret_cast<float*>(ws + 2 * row_region);
             both.front.pieces = reinterpret_cast<float*>(ws + 2 * row_region + own_bytes);
-            main_step(both.front, front_streams);
-            main_step(both.own, true);
-            step(3, both, a.tokens, a.kv_heads, 1, 256, 0);
+            main_step(both.front);
+            main_step(both.own);
+            step(4, both, a.tokens, a.kv_heads, 1, std::min(1024u, (a.group * dim / 4 + 63) / 64 * 64), 0);
             return 0;
         }
     }
     a.part = kWholeSequences;
     a.pieces = reinterpret_cast<float*>(ws);
-    lay_out(a, stream, dev.workspace_bytes);
+    lay_out(a, own_rows, dev.workspace_bytes);
     if (a.workgroups == 0) return bad("the workspace holds no part of a segment");
-    main_step(a, stream);
-    if (a.workgroups > 1) step(2, a, a.workgroups - 1, stream ? 2 : 8, 1, 256, 0);
+    main_step(a);
+    if (a.workgroups > 1) step(3, a, a.workgroups - 1, stream ? 2 : 8, 1, 256, 0);
     return 0;
 }
 

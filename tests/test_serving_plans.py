@@ -17,8 +17,8 @@ B = cc.bind
     ("rope_half_d256_r64", "smelt_rope_vec_f16"), ("rope_interleaved_d100_r20@bf16", "smelt_rope_vec_bf16"),
     ("paged_kv_append_half_d128_r0_kv8_p16", "smelt_paged_append_vec_f16"),
     ("paged_kv_append_q_interleaved_d64_r64_kv1_p256", "smelt_paged_append_vec_f16"),
-    ("paged_attention_d256_h24_kv4_p64", "smelt_attention_stream_d256_f16"),
-    ("paged_attention_shared_d64_h6_kv2_p16@bf16", "smelt_attention_stream_d64_p16_bf16"),
+    ("paged_attention_d256_h24_kv4_p64", "smelt_attention_stream16_d256_f16"),
+    ("paged_attention_shared_d64_h6_kv2_p16@bf16", "smelt_attention_stream16_d64_bf16"),
     ("verify_drafts", "smelt_verify_stats_f16"), ("verify_drafts_given@bf16", "smelt_verify_stats_bf16")])
 def test_names_resolve(name, symbol):
     rc, sym, kinds = cc.resolve_pipeline_name(name)
