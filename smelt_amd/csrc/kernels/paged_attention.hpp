@@ -602,22 +602,21 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
 }
 
 // Many rows (prompts, the prefix against a batch): bound by the matrix cores.  A workgroup's WAVES waves hold 32 rows each and walk
-// the key tiles together, in stages of NS tiles that are loaded from the cache straight to LDS (no registers in between) while the
-// BUFFERS - 1 stages before are waited for and worked on, one barrier a stage.  Every wave takes its operands from there: K in
-// operand order, V through the transposing LDS read (16 lanes take 4 keys x 16 values and get one value of 4 keys each), the
-// 16-byte pieces of V rows placed so that the four keys of such a read lie on different banks.
+// the key tiles of a run together, in stages of NS tiles that are loaded from the cache straight to LDS (no registers in between) while
+// the BUFFERS - 1 stages before are waited for and worked on, one barrier a stage.  Every load of a wave lies within one half tile
+// and so within one page: a scalar base (page ids are fetched a stage ahead) and offsets of the lanes that never change.  Every
+// wave takes its operands from LDS: K in operand order, V through the transposing LDS read (16 lanes take 4 keys x 16 values and
+// get one value of 4 keys each), the 16-byte pieces of V rows placed so that the four keys of such a read lie on different banks.
 typedef short attn_short4_t __attribute__((ext_vector_type(4)));
 constexpr int kAttnBuffers = 4;
-template <int D, int NS>
-struct AttnTilesShared { uint16_t tile[kAttnBuffers][NS][2][32 * D]; };      // K, V
 
-// 16-byte piece c of V row r lies at piece c ^ (4 * turn): of rows 4 apart in a read, on different banks
+// 16-byte piece c of V row r lies at piece c ^ (4 * turn): the rows of a read on different banks
 template <int D>
 __device__ __forceinline__ uint32_t attn_v_turn(uint32_t row) { return D == 64 ? (row >> 1) & 1u : row & 3u; }
 
-// 16 bytes a lane from `src` to LDS at `lds` + 16 * lane; counts as a vector load, in order
-__device__ __forceinline__ void attn_load_lds(const uint16_t* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+// 16 bytes a lane from base + offset to LDS at `lds` + 16 * lane; counts as a vector load, in order
+__device__ __forceinline__ void attn_load_lds(uint64_t base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 // waits until at most N of the wave's vector loads are under way
 template <int N>
@@ -626,9 +625,8 @@ __device__ __forceinline__ void attn_wait_loads() { asm volatile("s_waitcnt vmcn
 template <class ActT, int D, int WAVES, int NS>
 __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    AttnTilesShared<D, NS>& sh = *reinterpret_cast<AttnTilesShared<D, NS>*>(smem);
-    constexpr uint32_t R = 32 * WAVES, T = 64 * WAVES;
-    constexpr int P = 8 * D / T;                         // 16-byte pieces of a key tile (K, then V) that a thread loads
+    constexpr uint32_t R = 32 * WAVES, kHalf = 16 * D * 2, kTile = 4 * kHalf, kStage = NS * kTile;      // bytes: K halves, V halves
+    constexpr int P = D / (8 * WAVES), kPerHalf = D / 32;       // loads of a wave a tile; wave loads a half
     const AttnWork work = find_work<kFirstUnit>(a, blockIdx.x);
     if (work.entry == ~0u) return;
     uint32_t unit = work.at, index = work.entry, base = work.base;
@@ -636,9 +634,18 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, half = lane >> 5;
     const AttnScale scale = attn_scale(a);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem);
-    // the lane's share of a transposing read: key row and 8-byte piece; the pieces of 32 values further on are turned by the row
+    // the lane's place in each of the wave's loads: piece `at` of a half, K [dim / 8][key][8] or V [key][dim]
+    uint32_t offset[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const uint32_t q = p * WAVES + wave, at = (q % kPerHalf) * 64 + lane;
+        const uint32_t key = at / (D / 8), col = (at % (D / 8)) ^ (4 * attn_v_turn<D>(key));
+        offset[p] = q < 2 * kPerHalf ? ((at / 16 << a.page_shift) + at % 16) * 16 : (key * D + col * 8) * 2;
+    }
+    // ... and of a transposing read: key row and 8-byte piece; the pieces of 32 values further on are turned by the row
     const uint32_t v_row = 4 * half + (lane & 15) / 4, v_turn = attn_v_turn<D>(v_row);
     const uint32_t v_lane = v_row * 2 * D + ((lane & 31) / 16) * 32 + (lane & 3) * 8;
+    const uint32_t k_lane = ((lane & 31) / 16) * kHalf + half * 256 + (lane & 15) * 16;
 #pragma unroll 1
     while (unit < unit_end) {
         const AttentionEntry e = attn_entry(a, index);
@@ -647,120 +654,164 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
         else if (!attn_segment(a, e, base, unit, unit_end, g)) { base = g.begin; ++index; continue; }
         unit += g.units;
         if (g.first >= g.last) continue;                 // (only some of its lead)
-        const int32_t* own_table = a.page_table + (size_t)(e.sequence < 0 ? 0 : e.sequence) * a.pages_per_sequence;
-
-        uint32_t pages_known = 0;                         // four bits a buffer, two a tile: the tile's halves are on pages of the pool's
-        auto fetch = [&](uint32_t first, uint32_t buffer) {
-            pages_known &= ~(15u << (4 * buffer));
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                // (past the part's end: its last tile once more, so that every stage is the same number of loads)
-                uint32_t ct = first + n < g.last ? first + n : g.last - 1;
-                if (ct >= e.tiles) continue;             // (no keys at all)
-                const bool run = ct >= e.front_tiles;
-                const uint32_t tile = ct - (run ? e.front_tiles : 0u);
-                const AttnTile at = attn_tile<D>(a, run ? own_table : a.prefix_table, g.kv_head, run ? e.own : e.front, tile);
-                pages_known |= at.known << (4 * buffer + 2 * n);
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const uint32_t piece = p * T + threadIdx.x;
-                    const uint32_t lds = lds0 + (((buffer * NS + n) * 2) * 32 * D * 2) + (p * T + wave * 64) * 16;
-                    const uint16_t* src;
-                    if ((p * T + wave * 64) < 4 * D) {                                                       // K: [dim / 8][key][8]
-                        const uint32_t chunk = piece / 32, key = piece % 32;
-                        src = a.k_cache + (key < 16 ? at.page[0] : at.page[1]) + (((chunk << a.page_shift) + (key < 16 ? at.off[0] : at.off[1]) + (key & 15)) << 3);
-                    } else {                                                                                 // V: [key][dim]
-                        const uint32_t key = (piece - 4 * D) / (D / 8), col = ((piece - 4 * D) % (D / 8)) ^ (4 * attn_v_turn<D>(key));
-                        src = a.v_cache + (key < 16 ? at.page[0] : at.page[1]) + ((key < 16 ? at.off[0] : at.off[1]) + (key & 15)) * D + col * 8;
-                    }
-                    attn_load_lds(src, __builtin_amdgcn_readfirstlane(lds));
-                }
-            }
-        };
-        const uint32_t stages = (g.last - g.first + NS - 1) / NS;
-#pragma unroll 1
-        for (uint32_t s = 0; s < kAttnBuffers - 1 && s < stages; ++s) fetch(g.first + s * NS, s);
-
         const uint32_t row0 = g.row_tile * R + wave * 32;
         const AttnRow row = attn_row(a, e, row0 + (lane & 31));
         AttnAcc<D> acc;
         attn_clear<D>(acc);
         uint4_t qf[D / 16];
         attn_load_q<D / 16>(a, row, a.q + (size_t)row.token * a.q_stride + (size_t)(g.kv_head * a.group + row.head) * D + 8 * half, 16, qf);
-        const AttnBounds front_b = attn_bounds(a, row, 0, (int32_t)e.front), own_b = attn_bounds(a, row, (int32_t)e.prefix, (int32_t)e.own);
-        const AttnRun front = attn_run(a, e, 0, row0, 32, &front_b, 1), own = attn_run(a, e, 1, row0, 32, &own_b, 1);
-        attn_wait_loads<0>();                             // (the compiler counts q's loads alone: from here on only stages are under way)
+        const uint32_t page_bytes = (a.kv_heads * D * 2) << a.page_shift, head_bytes = (g.kv_head * D * 2) << a.page_shift;
+        const uint64_t k_base = (uint64_t)(uintptr_t)a.k_cache + head_bytes, v_base = (uint64_t)(uintptr_t)a.v_cache + head_bytes;
+#pragma unroll 1
+        for (int run = 0; run < 2; ++run) {
+            const uint32_t len = run ? e.own : e.front, tile0 = run ? e.front_tiles : 0u, tiles = (len + 31) / 32;
+            const uint32_t first = g.first > tile0 ? g.first - tile0 : 0u;
+            uint32_t last = g.last > tile0 ? g.last - tile0 : 0u;
+            last = last < tiles ? last : tiles;
+            if (first >= last) continue;
+            const scalar_table table = as_scalar(run ? a.page_table + (size_t)e.sequence * a.pages_per_sequence : a.prefix_table);
+            const uint32_t last_page = (len - 1) >> a.page_shift, page_mask = (1u << a.page_shift) - 1u;
+            const AttnBounds b = attn_bounds(a, row, run ? (int32_t)e.prefix : 0, (int32_t)len);
+            const AttnRun u = attn_run(a, e, run, row0, 32, &b, 1);
+            const uint32_t stages = (last - first + NS - 1) / NS;
+
+            // pages of a stage's half tiles; past the run's part its last tile once more, so that every stage is the same number of loads
+            struct Pages { uint32_t id[NS][2]; };
+            auto pages_of = [&](uint32_t stage) {
+                Pages p;
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t tile = first + stage * NS + n;
+                        tile = tile < last ? tile : last - 1;
+                        uint32_t i = (tile * 32 + 16 * h) >> a.page_shift;
+                        i = i < last_page ? i : last_page;      // behind the run: masked by its length
+                        p.id[n][h] = (uint32_t)table[__builtin_amdgcn_readfirstlane(i)];
+                    }
+                return p;
+            };
+            uint32_t pages_known = 0;                     // four bits a buffer, two a tile: the halves are on pages of the pool's
+            auto fetch = [&](uint32_t stage, const Pages& pages) {
+                const uint32_t buffer = stage % kAttnBuffers;
+                pages_known &= ~(15u << (4 * buffer));
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    uint32_t tile = first + stage * NS + n;
+                    tile = tile < last ? tile : last - 1;
+                    uint64_t at[2];
+                    uint32_t off[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const bool known = pages.id[n][h] < a.pages;
+                        pages_known |= known ? 1u << (4 * buffer + 2 * n + h) : 0u;
+                        at[h] = (uint64_t)(known ? pages.id[n][h] : 0u) * page_bytes;
+                        off[h] = (tile * 32 + 16 * h) & page_mask;
+                    }
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const uint32_t q = p * WAVES + wave, region = q / kPerHalf, h = region & 1;
+                        const uint64_t page = h ? at[1] : at[0];
+                        const uint32_t o = h ? off[1] : off[0];
+                        const uint64_t from = region < 2 ? k_base + page + o * 16 : v_base + page + o * (D * 2);
+                        attn_load_lds(from, offset[p], lds0 + buffer * kStage + n * kTile + q * 1024);
+                    }
+                }
+            };
+#pragma unroll 1
+            for (uint32_t s = 0; s < kAttnBuffers - 1 && s < stages; ++s) fetch(s, pages_of(s));
+            Pages pages = pages_of(kAttnBuffers - 1);
+            // (the compiler counts its own loads alone: from here on only stages are under way)
+            if (run == 0 || e.front_tiles == 0) attn_wait_loads<0>();
 
 #pragma unroll 1
-        for (uint32_t stage = 0; stage < stages; ++stage) {
-            const uint32_t first = g.first + stage * NS, buffer = stage % kAttnBuffers;
-            // this stage is complete when only the later ones' loads are left
-            if (stage + kAttnBuffers - 1 <= stages) attn_wait_loads<(kAttnBuffers - 2) * P * NS>();
-            else attn_wait_loads<0>();
-            __syncthreads();
-            const uint32_t stage_known = pages_known >> (4 * buffer);
-            if (stage + kAttnBuffers - 1 < stages) fetch(first + (kAttnBuffers - 1) * NS, (stage + kAttnBuffers - 1) % kAttnBuffers);
-            // what the wave's rows see of the stage, and what there is of it (a tile past the part's end: nothing)
-            bool seen = false, edge[NS], ragged = false;
-            uint32_t known[NS];
-            int32_t key0[NS];
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const uint32_t ct = first + n;
-                const bool some = ct < g.last && ct < e.tiles, run = ct >= e.front_tiles;
-                const AttnRun& u = run ? own : front;
-                const uint32_t tile = ct - (run ? e.front_tiles : 0u), len = run ? e.own : e.front;
-                key0[n] = (int32_t)tile * (int32_t)smelt_serving::kKeyTile;
-                known[n] = some ? (stage_known >> (2 * n)) & 3u : 0u;
-                seen = seen || (some && attn_seen(u, key0[n]));
-                edge[n] = known[n] != 3u || attn_masked(u, key0[n]);
-                ragged = ragged || known[n] != 3u || tile * 32 + 32 > len;
-            }
-            if (ragged) {
-                // Values of keys behind the run's end, or on a page that is none of the pool's, are whatever memory holds: zero them, since a
-                // zero probability does not silence an infinity or a NaN.
-#pragma unroll 1
-                for (int n = 0; n < NS; ++n) {
-                    const uint32_t len = first + n >= e.front_tiles ? e.own : e.front;
-                    uint4_t* v = reinterpret_cast<uint4_t*>(sh.tile[buffer][n][1]);
-                    for (uint32_t p = threadIdx.x; p < 4 * D; p += T) {
-                        const uint32_t key = p / (D / 8);
-                        if ((uint32_t)key0[n] + key >= len || !((known[n] >> (key / 16)) & 1u)) v[p] = uint4_t{0, 0, 0, 0};
-                    }
-                }
+            for (uint32_t stage = 0; stage < stages; ++stage) {
+                const uint32_t buffer = stage % kAttnBuffers;
+                // this stage is complete when only the later ones' loads are left
+                if (stage + kAttnBuffers - 1 <= stages) attn_wait_loads<(kAttnBuffers - 2) * P * NS>();
+                else attn_wait_loads<0>();
                 __syncthreads();
-            }
-            if (!seen) continue;
-            float16_t s[NS];
+                // what the wave's rows see of the stage, and what there is of it (a tile past the part's end: nothing)
+                bool seen = false, edge[NS], ragged = false;
+                uint32_t known[NS];
+                int32_t key0[NS];
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const uint4_t* kl = reinterpret_cast<const uint4_t*>(sh.tile[buffer][n][0]) + lane;
-                s[n] = attn_mfma<ActT>(kl[0], qf[0], float16_t{});
+                for (int n = 0; n < NS; ++n) {
+                    const uint32_t tile = first + stage * NS + n;
+                    const bool some = tile < last;
+                    key0[n] = (int32_t)tile * (int32_t)smelt_serving::kKeyTile;
+                    known[n] = some ? (pages_known >> (4 * buffer + 2 * n)) & 3u : 0u;
+                    seen = seen || (some && attn_seen(u, key0[n]));
+                    edge[n] = known[n] != 3u || attn_masked(u, key0[n]);
+                    ragged = ragged || known[n] != 3u || (uint32_t)key0[n] + 32 > len;
+                }
+                const unsigned char* st = smem + buffer * kStage;
+                if (ragged) {
+                    // Values of keys behind the run's end, or on a page that is none of the pool's, are whatever memory holds: zero them,
+                    // since a zero probability does not silence an infinity or a NaN.
+#pragma unroll 1
+                    for (int n = 0; n < NS; ++n) {
+                        uint4_t* v = reinterpret_cast<uint4_t*>(smem + buffer * kStage + n * kTile + 2 * kHalf);
+                        for (uint32_t p = threadIdx.x; p < 4 * D; p += 64 * WAVES) {
+                            const uint32_t key = p / (D / 8);
+                            if ((uint32_t)key0[n] + key >= len || !((known[n] >> (key / 16)) & 1u)) v[p] = uint4_t{0, 0, 0, 0};
+                        }
+                    }
+                    __syncthreads();
+                }
+                // operands are read well before the products that take them: K of a tile while the one before is multiplied, V before the softmax
+                float16_t s[NS];
+                if (seen) {
+                    uint4_t kf[2][D / 16];
+                    auto load_k = [&](int n) {
+                        const uint4_t* kl = reinterpret_cast<const uint4_t*>(st + n * kTile + k_lane);
 #pragma unroll
-                for (int d = 1; d < D / 16; ++d) s[n] = attn_mfma<ActT>(kl[d * 64], qf[d], s[n]);
-            }
+                        for (int d = 0; d < D / 16; ++d) kf[n & 1][d] = kl[d * 32];
+                    };
+                    load_k(0);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-                if (edge[n]) attn_hide(s[n], key0[n], first + n >= e.front_tiles ? own_b : front_b, known[n]);
-            attn_softmax<D, NS>(scale, acc, s);
+                    for (int n = 0; n < NS; ++n) {
+                        if (n + 1 < NS) { load_k(n + 1); __builtin_amdgcn_sched_barrier(0); }
+                        s[n] = attn_mfma<ActT>(kf[n & 1][0], qf[0], float16_t{});
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const char* vl = reinterpret_cast<const char*>(sh.tile[buffer][n][1]) + v_lane;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint4_t pf = attn_pack<ActT>(s[n], u);
-#pragma unroll
-                    for (int j = 0; j < D / 32; ++j) {
-                        const char* at = vl + 16 * u * 2 * D + ((j & ~3) | ((j & 3) ^ v_turn)) * 64;
-                        typedef __attribute__((address_space(3))) attn_short4_t* lds_ptr;
-                        const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at));
-                        const uint2_t hi = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 8 * 2 * D)));
-                        acc.o[j] = attn_mfma<ActT>(uint4_t{lo.x, lo.y, hi.x, hi.y}, pf, acc.o[j]);
+                        for (int d = 1; d < D / 16; ++d) s[n] = attn_mfma<ActT>(kf[n & 1][d], qf[d], s[n]);
                     }
                 }
+                if (stage + kAttnBuffers - 1 < stages) {
+                    fetch(stage + kAttnBuffers - 1, pages);
+                    pages = pages_of(stage + kAttnBuffers);
+                }
+                if (!seen) continue;
+                uint4_t vf[NS][2][D / 32];
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < D / 32; ++j) {
+                            const unsigned char* at = st + n * kTile + 2 * kHalf + v_lane + h * kHalf + ((j & ~3) | ((j & 3) ^ v_turn)) * 64;
+                            typedef __attribute__((address_space(3))) attn_short4_t* lds_ptr;
+                            const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at));
+                            const uint2_t hi = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 8 * 2 * D)));
+                            vf[n][h][j] = uint4_t{lo.x, lo.y, hi.x, hi.y};
+                        }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+                    if (edge[n]) attn_hide(s[n], key0[n], b, known[n]);
+                attn_softmax<D, NS>(scale, acc, s);
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint4_t pf = attn_pack<ActT>(s[n], h);
+#pragma unroll
+                        for (int j = 0; j < D / 32; ++j) acc.o[j] = attn_mfma<ActT>(vf[n][h][j], pf, acc.o[j]);
+                    }
             }
+            __syncthreads();                              // (the next loads overwrite the stages)
         }
-        __syncthreads();                                  // (the next part's loads overwrite the stages)
         // a lane holds its row's values 32 j + 8 (i / 4) + 4 half + i % 4
         float* piece = a.pieces + ((size_t)blockIdx.x * 2 + (g.first == g.tiles.lo ? 1 : 0)) * smelt_serving::piece_floats(R, D);
         const float l = attn_halves_sum(acc.l);
