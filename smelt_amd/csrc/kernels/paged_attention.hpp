@@ -71,24 +71,21 @@ __device__ __forceinline__ scalar_table as_scalar(const int32_t* p) { return (sc
 struct AttnScalarLoad { __device__ __forceinline__ int32_t operator()(const int32_t* p, uint32_t i) const { return as_scalar(p)[__builtin_amdgcn_readfirstlane(i)]; } };
 __device__ __forceinline__ AttentionEntry attn_entry(const AttentionArgs& a, uint32_t index) { return smelt_serving::attention_entry(a, index, AttnScalarLoad()); }
 
-// What a workgroup looks for: its first unit (or its segment), the first unit of the workgroup after it, or the entry of a token.
-enum AttnWanted { kFirstUnit, kCut, kToken };
+// Where a workgroup begins.
 struct AttnWork {
     AttentionSplit split;    // of the whole launch
-    uint32_t entry;          // where the wanted unit, segment or row lies (~0: nowhere)
+    uint32_t entry;          // where its first unit (its segment) lies, ~0: nowhere
     uint32_t base;           // units (segments where each workgroup takes one) before that entry
-    uint32_t at;             // the wanted unit (segment)
+    uint32_t at;             // the unit (segment)
 };
 
 // Each wave looks for itself (no barrier), an entry a lane: once through the entries for their total, then for the wanted one.
-template <AttnWanted WANTED>
-__device__ __forceinline__ AttnWork find_work(const AttentionArgs& a, uint32_t want) {
+__device__ __forceinline__ AttnWork find_work(const AttentionArgs& a, uint32_t group) {
     const uint32_t entries = smelt_serving::attention_entries(a), lane = threadIdx.x % kWave;
     AttnWork w;
     w.entry = ~0u;
     w.base = w.at = 0;
     uint32_t mine[2] = {0, 0}, before[2] = {0, 0}, all[2] = {0, 0};      // units and segments: the lane's entry, the entries before it in the round, the round's
-    bool here = false;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
         uint32_t run[2] = {0, 0};
@@ -97,12 +94,10 @@ __device__ __forceinline__ AttnWork find_work(const AttentionArgs& a, uint32_t w
             const uint32_t index = base + lane;
             if (pass == 0 || entries > (uint32_t)kWave) {
                 mine[0] = mine[1] = 0;
-                here = false;
                 if (index < entries) {
                     const AttentionEntry e = smelt_serving::attention_entry(a, index);
                     mine[0] = smelt_serving::attention_units(a, e);
                     mine[1] = smelt_serving::attention_segments(a, e);
-                    here = want >= e.first_token && want - e.first_token < e.tokens;
                 }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -119,8 +114,7 @@ __device__ __forceinline__ AttnWork find_work(const AttentionArgs& a, uint32_t w
             if (pass == 1) {
                 const int k = w.split.whole ? 1 : 0;
                 const uint32_t first = run[k] + before[k];
-                const bool ok = WANTED == kToken ? here : w.at >= first && w.at - first < mine[k];
-                const unsigned long long who = __ballot(ok);
+                const unsigned long long who = __ballot(w.at >= first && w.at - first < mine[k]);
                 if (who) {
                     const int from = __builtin_ctzll(who);
                     w.entry = __builtin_amdgcn_readfirstlane(base + from);
@@ -133,11 +127,8 @@ __device__ __forceinline__ AttnWork find_work(const AttentionArgs& a, uint32_t w
         }
         if (pass == 1) break;
         w.split = smelt_serving::attention_split(a, run[0], run[1]);
-        if (WANTED != kToken) {
-            const uint32_t group = want + (WANTED == kCut ? 1u : 0u);
-            if (group >= w.split.groups || (WANTED == kCut && w.split.whole)) return w;
-            w.at = w.split.whole ? group : smelt_serving::attention_start(w.split, group);
-        }
+        if (group >= w.split.groups) return w;
+        w.at = w.split.whole ? group : smelt_serving::attention_start(w.split, group);
     }
     return w;
 }
@@ -181,6 +172,30 @@ __device__ __forceinline__ void attn_whole_segment(const AttentionArgs& a, const
     g.whole = true;
     g.begin = 0;
     g.units = 1;
+}
+
+// the slot of the part of a segment that workgroup w leaves
+__device__ __forceinline__ float* attn_piece(const AttentionArgs& a, const AttnSegment& g, uint32_t dim) {
+    const uint32_t slot = a.by_segment ? blockIdx.x + g.row_tile * a.kv_heads + g.kv_head : 2 * blockIdx.x + (g.first == g.tiles.lo ? 1u : 0u);
+    return a.pieces + (size_t)slot * smelt_serving::piece_floats(a.row_tile, dim);
+}
+// the last workgroup that has a part of a segment
+__device__ __forceinline__ uint32_t attn_last(const AttentionSplit& split, const AttnSegment& g) {
+    return smelt_serving::attention_owner(split, g.begin + (g.tiles.hi - g.tiles.lo) - 1);
+}
+// kWholeSequences: the workgroup's note for the join (every workgroup leaves one: none at its start, overwritten by the same thread)
+__device__ __forceinline__ void attn_note_cut(const AttentionArgs& a, const smelt_serving::AttentionCut& cut) {
+    if (a.part == smelt_serving::kWholeSequences && blockIdx.x < a.workgroups && threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
+}
+__device__ __forceinline__ smelt_serving::AttentionCut attn_cut(const AttentionArgs& a, const AttentionEntry& e, const AttentionSplit& split, const AttnSegment& g) {
+    const uint32_t row0 = g.row_tile * a.row_tile, left = e.tokens * a.group - row0;
+    return {attn_last(split, g), g.kv_head, e.first_token, row0, left < a.row_tile ? left : a.row_tile, {0, 0, 0}};
+}
+// kOwnKeys, kPrefix: ends a row (r within its tile) of a segment that begins here
+__device__ __forceinline__ void attn_end_row(float* end, const AttentionArgs& a, const AttentionSplit& split, const AttnSegment& g, uint32_t r, float max, float sum) {
+    const uint32_t parts = g.whole ? 1u : attn_last(split, g) - blockIdx.x + 1u;
+    const uint32_t slot = a.by_segment ? blockIdx.x + g.row_tile * a.kv_heads + g.kv_head : 2 * blockIdx.x + 1;
+    *reinterpret_cast<smelt_serving::AttentionRowEnd*>(end) = smelt_serving::AttentionRowEnd{max, sum, slot, parts << 8 | r};
 }
 
 // the sequence of a token row: offsets is ascending, tokens before offsets[sequences] belong to one
@@ -410,7 +425,8 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
     AttnShared<D, RT>& sh = *reinterpret_cast<AttnShared<D, RT>*>(smem);
     constexpr uint32_t R = 16 * RT;
     constexpr int KS = D / 32, VE = D == 64 ? 4 : 8, VC = D == 256 ? 2 : 1, MT = D / 16;   // k steps of a score; values a lane takes of a V row, in VC pieces; tiles of 16 values
-    const AttnWork work = find_work<kFirstUnit>(a, blockIdx.x);
+    const AttnWork work = find_work(a, blockIdx.x);
+    attn_note_cut(a, {});
     if (work.entry == ~0u) return;
     uint32_t unit = work.at, index = work.entry, base = work.base;
     const uint32_t unit_end = smelt_serving::attention_start(work.split, blockIdx.x + 1);
@@ -569,7 +585,9 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
         }
         __syncthreads();
         const uint32_t rows_live = e.tokens * a.group - row0 < R ? e.tokens * a.group - row0 : R;
-        float* piece = a.pieces + ((size_t)blockIdx.x * 2 + (g.first == g.tiles.lo ? 1 : 0)) * smelt_serving::piece_floats(R, D);
+        const bool begins = g.first == g.tiles.lo;
+        if (begins && !g.whole) attn_note_cut(a, attn_cut(a, e, work.split, g));
+        float* piece = attn_piece(a, g, D);
 #pragma unroll 1
         for (uint32_t item = threadIdx.x; item < rows_live * (D / 4); item += blockDim.x) {
             const uint32_t r = item / (D / 4), d = (item % (D / 4)) * 4;
@@ -585,13 +603,13 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
                 sum += f * sh.l[w][r];
             }
             const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
+            float* dst = attn_whole_row(a, token, head, D);
+            if (a.part != smelt_serving::kWholeSequences && begins && d == 0) attn_end_row(dst + D, a, work.split, g, r, top, sum);
             if (!g.whole) {
                 *reinterpret_cast<float4_t*>(piece + 2 * R + r * D + d) = y;
                 if (d == 0) { piece[r] = top; piece[R + r] = sum; }
             } else if (a.part != smelt_serving::kWholeSequences) {
-                float* dst = attn_whole_row(a, token, head, D);
                 *reinterpret_cast<float4_t*>(dst + d) = y;
-                if (d == 0) { dst[D] = top; dst[D + 1] = sum; }
             } else {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 *reinterpret_cast<uint2_t*>(a.out + ((size_t)token * a.heads + head) * D + d) = uint2_t{attn_pack2<ActT>(y.x * inv, y.y * inv), attn_pack2<ActT>(y.z * inv, y.w * inv)};
@@ -627,7 +645,8 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr uint32_t R = 32 * WAVES, kHalf = 16 * D * 2, kTile = 4 * kHalf, kStage = NS * kTile;      // bytes: K halves, V halves
     constexpr int P = D / (8 * WAVES), kPerHalf = D / 32;       // loads of a wave a tile; wave loads a half
-    const AttnWork work = find_work<kFirstUnit>(a, blockIdx.x);
+    const AttnWork work = find_work(a, blockIdx.x);
+    attn_note_cut(a, {});
     if (work.entry == ~0u) return;
     uint32_t unit = work.at, index = work.entry, base = work.base;
     const uint32_t unit_end = work.split.whole ? unit + 1 : smelt_serving::attention_start(work.split, blockIdx.x + 1);
@@ -813,7 +832,9 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
             __syncthreads();                              // (the next loads overwrite the stages)
         }
         // a lane holds its row's values 32 j + 8 (i / 4) + 4 half + i % 4
-        float* piece = a.pieces + ((size_t)blockIdx.x * 2 + (g.first == g.tiles.lo ? 1 : 0)) * smelt_serving::piece_floats(R, D);
+        const bool begins = g.first == g.tiles.lo;
+        if (begins && !g.whole) attn_note_cut(a, attn_cut(a, e, work.split, g));
+        float* piece = attn_piece(a, g, D);
         const float l = attn_halves_sum(acc.l);
         if (row.live) {
             const uint32_t r = wave * 32 + (lane & 31), head = g.kv_head * a.group + row.head;
@@ -827,10 +848,11 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                         *reinterpret_cast<uint2_t*>(out + 32 * j + 2 * i) = uint2_t{attn_pack2<ActT>(acc.o[j][i] * inv, acc.o[j][i + 1] * inv),
                                                                                    attn_pack2<ActT>(acc.o[j][i + 2] * inv, acc.o[j][i + 3] * inv)};
             } else {
-                float* dst = g.whole ? attn_whole_row(a, row.token, head, D) : piece + 2 * R + r * D;
+                float* whole = attn_whole_row(a, row.token, head, D);
+                float* dst = g.whole ? whole : piece + 2 * R + r * D;
                 if (half == 0) {
-                    if (g.whole) { dst[D] = acc.m; dst[D + 1] = l; }
-                    else { piece[r] = acc.m; piece[R + r] = l; }
+                    if (a.part != smelt_serving::kWholeSequences && begins) attn_end_row(whole + D, a, work.split, g, r, acc.m, l);
+                    if (!g.whole) { piece[r] = acc.m; piece[R + r] = l; }
                 }
 #pragma unroll
                 for (int j = 0; j < D / 32; ++j)
@@ -851,25 +873,27 @@ __device__ __forceinline__ void attn_join(AttnJoin& j, float m, float l, float4_
     j.l = f * j.l + g * l;
     j.m = top;
 }
-// row r of the segment's parts that workgroups w0 .. w1 left
+// row r of `parts` parts of a segment, the first in slot `first`
 template <int D>
-__device__ __forceinline__ void attn_join_pieces(AttnJoin& j, const AttentionArgs& a, const AttentionSplit& split, uint32_t begin, uint32_t w0, uint32_t w1, uint32_t r, uint32_t d, float c) {
+__device__ __forceinline__ void attn_join_pieces(AttnJoin& j, const AttentionArgs& a, uint32_t first, uint32_t parts, uint32_t r, uint32_t d, float c) {
     constexpr uint32_t U = 8;      // parts whose loads are under way together
-    for (uint32_t base = w0; base <= w1; base += U) {
+#pragma unroll 1
+    for (uint32_t base = 0; base < parts; base += U) {
         float m[U], l[U];
         float4_t y[U];
 #pragma unroll
         for (uint32_t k = 0; k < U; ++k) {
-            const uint32_t w = base + k <= w1 ? base + k : w1;
-            const uint32_t slot = smelt_serving::attention_start(split, w) <= begin ? 1u : 0u;
-            const float* piece = a.pieces + ((size_t)w * 2 + slot) * smelt_serving::piece_floats(a.row_tile, D);
+            const uint32_t w = base + k < parts ? base + k : parts - 1;
+            uint32_t slot = a.by_segment ? first + w : (w ? 2 * (first / 2 + w) : first);
+            slot = slot < a.slots ? slot : a.slots - 1;
+            const float* piece = a.pieces + (size_t)slot * smelt_serving::piece_floats(a.row_tile, D);
             m[k] = piece[r];
             l[k] = piece[a.row_tile + r];
             y[k] = *reinterpret_cast<const float4_t*>(piece + 2 * a.row_tile + r * D + d);
         }
 #pragma unroll
         for (uint32_t k = 0; k < U; ++k)
-            if (base + k <= w1) attn_join(j, m[k], l[k], y[k], c);
+            if (base + k < parts) attn_join(j, m[k], l[k], y[k], c);
     }
 }
 template <class ActT>
@@ -881,24 +905,19 @@ __device__ __forceinline__ void attn_finish(const AttnJoin& j, uint16_t* out) {
     *reinterpret_cast<uint2_t*>(out) = w;
 }
 
-// kWholeSequences.  Grid: cuts between workgroups x slices of a segment's rows.  The first cut inside a segment stands for it.
+// kWholeSequences.  Grid: workgroups of the first launch x slices of a segment's rows.
 template <class ActT, int D>
 __device__ __forceinline__ void attn_combine(const AttentionArgs& a) {
-    const AttnWork work = find_work<kCut>(a, blockIdx.x);
-    if (work.entry == ~0u) return;
-    const AttentionEntry e = attn_entry(a, work.entry);
-    AttnSegment g;
-    if (!attn_segment(a, e, work.base, work.at, ~0u, g)) return;
-    const uint32_t end = g.begin + (g.tiles.hi - g.tiles.lo);
-    if (work.at <= g.begin || smelt_serving::attention_start(work.split, blockIdx.x) > g.begin) return;     // not inside a segment, or not the first
-    const uint32_t w1 = smelt_serving::attention_owner(work.split, end - 1);
-    const uint32_t row0 = g.row_tile * a.row_tile, left = e.tokens * a.group - row0, rows = left < a.row_tile ? left : a.row_tile;
+    typedef const __attribute__((address_space(4))) smelt_serving::AttentionCut* scalar_cut;
+    const scalar_cut c = (scalar_cut)(uintptr_t)(a.cuts + blockIdx.x);
+    const uint32_t last = c->last, kv_head = c->kv_head, first_token = c->first_token, row0 = c->row0, rows = c->rows;
+    if (last == 0) return;
 #pragma unroll 1
     for (uint32_t item = blockIdx.y * blockDim.x + threadIdx.x; item < rows * (D / 4); item += gridDim.y * blockDim.x) {
         const uint32_t r = item / (D / 4), d = (item % (D / 4)) * 4;
         AttnJoin j{-__builtin_inff(), 0.0f, {0, 0, 0, 0}};
-        attn_join_pieces<D>(j, a, work.split, g.begin, blockIdx.x, w1, r, d, a.scale_log2);
-        const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
+        attn_join_pieces<D>(j, a, 2 * blockIdx.x + 1, last - blockIdx.x + 1, r, d, a.scale_log2);
+        const uint32_t i = (row0 + r) / a.group, token = first_token + i, head = kv_head * a.group + (row0 + r) - i * a.group;
         attn_finish<ActT>(j, a.out + ((size_t)token * a.heads + head) * D + d);
     }
 }
@@ -906,38 +925,30 @@ __device__ __forceinline__ void attn_combine(const AttentionArgs& a) {
 // kPrefix and kOwnKeys.  Grid: tokens x kv heads: a row's two halves, each in parts or whole.
 template <class ActT, int D>
 __device__ __forceinline__ void attn_combine_shared(const smelt_serving::AttentionJoinArgs& both) {
+    const AttentionArgs& own = both.own;
     const uint32_t token = blockIdx.x, kv_head = blockIdx.y;
-    AttnWork work[2];
-    work[1] = find_work<kToken>(both.own, token);
-    if (work[1].entry == ~0u) return;       // a row behind the last sequence
-    work[0] = find_work<kToken>(both.front, token);
-    const uint32_t group = both.own.group;
+    if (token >= smelt_serving::clamp_count(as_scalar(own.offsets)[own.sequences], own.tokens)) return;     // a row behind the last sequence
+    const bool prefix = as_scalar(own.prefix_len)[0] > 0;
 #pragma unroll 1
-    for (uint32_t item = threadIdx.x; item < group * (D / 4); item += blockDim.x) {
-        const uint32_t g = item / (D / 4), d = (item % (D / 4)) * 4, head = kv_head * group + g;
+    for (uint32_t item = threadIdx.x; item < own.group * (D / 4); item += blockDim.x) {
+        const uint32_t head = kv_head * own.group + item / (D / 4), d = (item % (D / 4)) * 4;
+        const float* front_row = attn_whole_row(both.front, token, head, D);
+        const float* own_row = attn_whole_row(own, token, head, D);
+        const smelt_serving::AttentionRowEnd front_end = *reinterpret_cast<const smelt_serving::AttentionRowEnd*>(front_row + D);
+        const smelt_serving::AttentionRowEnd own_end = *reinterpret_cast<const smelt_serving::AttentionRowEnd*>(own_row + D);
+        const float4_t front_y = *reinterpret_cast<const float4_t*>(front_row + d), own_y = *reinterpret_cast<const float4_t*>(own_row + d);
         AttnJoin j{-__builtin_inff(), 0.0f, {0, 0, 0, 0}};
-#pragma unroll 1
-        for (int k = 0; k < 2; ++k) {
-            const AttentionArgs& x = k ? both.own : both.front;
-            const AttnWork w = k ? work[1] : work[0];
-            if (w.entry == ~0u) continue;       // no prefix
-            const AttentionEntry e = attn_entry(x, w.entry);
-            const uint32_t flat = (token - e.first_token) * group + g, row_tile = flat / x.row_tile, r = flat % x.row_tile;
-            uint32_t begin = w.base;
-            AttentionTiles s = smelt_serving::attention_tiles(x, e, 0);
-#pragma unroll 1
-            for (uint32_t t = 1; t <= row_tile; ++t) { begin += (s.hi - s.lo + x.lead) * x.kv_heads; s = smelt_serving::attention_tiles(x, e, t); }
-            begin += (s.hi - s.lo + x.lead) * kv_head + x.lead;
-            uint32_t w0 = 0, w1 = 0;
-            if (!w.split.whole) { w0 = smelt_serving::attention_owner(w.split, begin); w1 = smelt_serving::attention_owner(w.split, begin + (s.hi - s.lo) - 1); }
-            if (w0 == w1) {
-                const float* row = attn_whole_row(x, token, head, D);
-                attn_join(j, row[D], row[D + 1], *reinterpret_cast<const float4_t*>(row + d), x.scale_log2);
-            } else {
-                attn_join_pieces<D>(j, x, w.split, begin, w0, w1, r, d, x.scale_log2);
-            }
-        }
-        attn_finish<ActT>(j, both.own.out + ((size_t)token * both.own.heads + head) * D + d);
+        auto join = [&](const AttentionArgs& x, const smelt_serving::AttentionRowEnd& end, float4_t y) {
+            // (offsets that do not ascend leave rows without a segment: whatever is there stays within the slots)
+            uint32_t parts = end.parts_row >> 8, r = end.parts_row & 255u;
+            parts = parts < x.workgroups ? parts : x.workgroups;
+            r = r < x.row_tile ? r : x.row_tile - 1;
+            if (parts <= 1) attn_join(j, end.max, end.sum, y, x.scale_log2);
+            else attn_join_pieces<D>(j, x, end.piece < x.slots ? end.piece : 0u, parts, r, d, x.scale_log2);
+        };
+        if (prefix) join(both.front, front_end, front_y);
+        join(own, own_end, own_y);
+        attn_finish<ActT>(j, own.out + ((size_t)token * own.heads + head) * D + d);
     }
 }
 

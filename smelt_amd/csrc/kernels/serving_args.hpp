@@ -49,6 +49,20 @@ struct RopeArgs {
 constexpr uint32_t kKeyTile = 32;
 enum AttentionPart : uint32_t { kWholeSequences = 0, kOwnKeys = 1, kPrefix = 2 };
 
+// A segment whose parts several workgroups left, noted under the number of the first of them, whose part begins it.
+struct AttentionCut {
+    uint32_t last;                 // the last of the workgroups, 0: the workgroup begins no such segment
+    uint32_t kv_head, first_token, row0, rows;   // rows row0 .. row0 + rows of the entry that has its tokens from first_token on
+    uint32_t unused[3];
+};
+
+// Ends a row of AttentionArgs::rows: of a segment that one workgroup finished, or where the parts of it are.
+struct alignas(16) AttentionRowEnd {
+    float max, sum;
+    uint32_t piece;                // the first part's slot
+    uint32_t parts_row;            // parts << 8 | row within the tile
+};
+
 struct AttentionArgs {
     const uint16_t* q = nullptr;
     const uint16_t* k_cache = nullptr;
@@ -59,12 +73,15 @@ struct AttentionArgs {
     const int32_t* prefix_table = nullptr;
     const int32_t* prefix_len = nullptr;
     uint16_t* out = nullptr;
-    float* pieces = nullptr;       // two slots a workgroup: [row_tile] max, [row_tile] sum, [row_tile][dim]
-    float* rows = nullptr;         // not kWholeSequences: whole segments, a row of (dim + 4) a (token, head): [dim], max, sum
+    float* pieces = nullptr;       // slots of [row_tile] max, [row_tile] sum, [row_tile][dim]
+    float* rows = nullptr;         // not kWholeSequences: [dim] and an AttentionRowEnd a (token, head)
+    AttentionCut* cuts = nullptr;  // kWholeSequences: one a workgroup
     uint32_t tokens = 0, sequences = 0, heads = 0, kv_heads = 0, group = 0;
     uint32_t pages = 0, page_shift = 0, pages_per_sequence = 0, prefix_pages = 0;
     uint32_t window = 0, q_stride = 0, workgroups = 0, part = 0;
     uint32_t row_tile = 0;
+    uint32_t by_segment = 0;       // a part's slot: workgroup + segment (one entry), or else 2 * workgroup, + 1 for one that begins its segment
+    uint32_t slots = 0;
     uint32_t lead = 0;             // what beginning a segment costs, in key tiles
     uint32_t least_units = 1;      // a workgroup takes at least this many units
     uint32_t whole_from = ~0u;     // segments from which on each workgroup takes one

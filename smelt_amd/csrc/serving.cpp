@@ -282,21 +282,25 @@ int Planner::attention() {
     const bool stream = rows <= (uint64_t)32 * a.sequences;
     const uint32_t tile_rows = dim == 256 ? 128 : 256;
     auto row_tile = [&](uint64_t of, uint64_t over) { return of <= 16 * over ? 16u : (of <= 32 * over ? 32u : tile_rows); };
-    // The parts of cut segments live in the context's workspace: two a workgroup; with the prefix apart, so do the rows
-    // of segments that one workgroup finished.
-    auto slot_bytes = [&](uint32_t r) { return (size_t)piece_floats(r, dim) * 4 * 2; };
+    // The parts of cut segments live in the context's workspace, a workgroup leaving two at most (of its first and its last segment).
+    // Against the prefix, whose tiles are large, the parts are counted along workgroups and segments instead, where that is fewer.
     const size_t row_region = (size_t)a.tokens * a.heads * (dim + 4) * 4;
-    char* ws = static_cast<char*>(dev.workspace);
+    auto piece_bytes = [&](uint32_t r) { return (size_t)piece_floats(r, dim) * 4; };
     auto lay_out = [&](AttentionArgs& x, uint32_t r, size_t room) {
         x.row_tile = r;
         x.lead = kSegmentLead;
         x.least_units = x.lead + (r <= 32 ? 4 : 8);       // a key tile for each of four waves; stages to keep under way
         // workgroups that the register file holds
         const uint32_t per_cu = r == 16 ? (dim == 256 ? 2 : (dim == 128 ? 3 : 4)) : (r == 32 && dim != 256 ? 2 : 1);
-        x.workgroups = (uint32_t)std::min<size_t>((size_t)dev.compute_units * per_cu, room / slot_bytes(r));
+        const size_t most = (size_t)dev.compute_units * per_cu, slots = room / piece_bytes(r);
+        const uint64_t segments = (rows + r - 1) / r * a.kv_heads;
+        x.by_segment = x.part == kPrefix && segments < most && segments < slots / 2;
+        x.workgroups = (uint32_t)std::min<size_t>(most, x.by_segment ? slots - segments : slots / 2);
+        x.slots = x.by_segment ? x.workgroups + (uint32_t)segments : 2 * x.workgroups;
         // a segment each from three quarters of the workgroups on: no parts to write and join
         x.whole_from = r <= 32 ? ~0u : std::max(1u, dev.compute_units * 3 / 4);
     };
+    char* ws = static_cast<char*>(dev.workspace);
     auto main_step = [&](const AttentionArgs& x) {
         const uint32_t r = x.row_tile;
         if (r <= 32) {
@@ -312,7 +316,7 @@ int Planner::attention() {
     const uint64_t row_tiles = rows / 16 + a.sequences + 1;
     if (row_tiles * a.kv_heads > 0x7FFFFFFFull / (key_tiles + kSegmentLead)) return bad("rows times keys pass 2^31 key tiles");
     const uint32_t own_rows = row_tile(rows, a.sequences), front_rows = row_tile(rows, 1);
-    if (stream && shared && a.prefix_pages && 2 * row_region + slot_bytes(own_rows) + slot_bytes(front_rows) <= dev.workspace_bytes) {
+    if (stream && shared && a.prefix_pages && 2 * row_region <= dev.workspace_bytes) {
         AttentionJoinArgs both;
         both.front = a; both.own = a;
         both.front.part = kPrefix; both.own.part = kOwnKeys;
@@ -320,7 +324,7 @@ int Planner::attention() {
         both.own.rows = reinterpret_cast<float*>(ws + row_region);
         const size_t room = dev.workspace_bytes - 2 * row_region;
         lay_out(both.own, own_rows, room / 2);
-        const size_t own_bytes = (size_t)both.own.workgroups * slot_bytes(own_rows);
+        const size_t own_bytes = both.own.slots * piece_bytes(own_rows);
         lay_out(both.front, front_rows, room - own_bytes);
         if (both.own.workgroups && both.front.workgroups) {
             both.own.pieces = reinterpret_cast<float*>(ws + 2 * row_region);
@@ -332,8 +336,11 @@ int Planner::attention() {
         }
     }
     a.part = kWholeSequences;
-    a.pieces = reinterpret_cast<float*>(ws);
-    lay_out(a, own_rows, dev.workspace_bytes);
+    const size_t note_bytes = (size_t)dev.compute_units * 4 * sizeof(AttentionCut);       // (four workgroups a compute unit at most)
+    if (dev.workspace_bytes < note_bytes) return bad("the workspace holds no part of a segment");
+    a.cuts = reinterpret_cast<AttentionCut*>(ws);
+    a.pieces = reinterpret_cast<float*>(ws + note_bytes);
+    lay_out(a, own_rows, dev.workspace_bytes - note_bytes);
     if (a.workgroups == 0) return bad("the workspace holds no part of a segment");
     main_step(a);
     if (a.workgroups > 1) step(3, a, a.workgroups - 1, stream ? 2 : 8, 1, 256, 0);
