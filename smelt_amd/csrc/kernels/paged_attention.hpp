@@ -77,6 +77,7 @@ struct AttnWork {
     uint32_t entry;          // where its first unit (its segment) lies, ~0: nowhere
     uint32_t base;           // units (segments where each workgroup takes one) before that entry
     uint32_t at;             // the unit (segment)
+    uint32_t parts;          // kPrefix: of each segment
 };
 
 // Each wave looks for itself (no barrier), an entry a lane: once through the entries for their total, then for the wanted one.
@@ -84,7 +85,14 @@ __device__ __forceinline__ AttnWork find_work(const AttentionArgs& a, uint32_t g
     const uint32_t entries = smelt_serving::attention_entries(a), lane = threadIdx.x % kWave;
     AttnWork w;
     w.entry = ~0u;
-    w.base = w.at = 0;
+    w.base = w.at = w.parts = 0;
+    w.split = AttentionSplit{0, 0, 0, 0, false};
+    if (a.part == smelt_serving::kPrefix) {
+        const AttentionEntry e = attn_entry(a, 0);
+        w.parts = smelt_serving::attention_parts(a, e);
+        if (smelt_serving::attention_job(a, e, w.parts, group).some) w.entry = 0;
+        return w;
+    }
     uint32_t mine[2] = {0, 0}, before[2] = {0, 0}, all[2] = {0, 0};      // units and segments: the lane's entry, the entries before it in the round, the round's
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
@@ -141,6 +149,7 @@ struct AttnSegment {
     bool whole;
     uint32_t begin;              // the unit of the segment's first key tile
     uint32_t units;              // of the workgroup's run that lie in the segment
+    uint32_t slot;               // of the part
 };
 // the segment that holds unit `unit` of entry e, whose units start at `base`; false (and g.begin behind them) when the entry has fewer
 __device__ __forceinline__ bool attn_segment(const AttentionArgs& a, const AttentionEntry& e, uint32_t base, uint32_t unit, uint32_t unit_end, AttnSegment& g) {
@@ -158,6 +167,7 @@ __device__ __forceinline__ bool attn_segment(const AttentionArgs& a, const Atten
         g.first = g.tiles.lo + (done > a.lead ? done - a.lead : 0u);
         g.last = g.tiles.lo + (done + g.units > a.lead ? done + g.units - a.lead : 0u);
         g.whole = g.first == g.tiles.lo && g.last == g.tiles.hi;
+        g.slot = 2 * blockIdx.x + (g.first == g.tiles.lo ? 1u : 0u);
         return true;
     }
     return false;
@@ -170,14 +180,26 @@ __device__ __forceinline__ void attn_whole_segment(const AttentionArgs& a, const
     g.first = g.tiles.lo;
     g.last = g.tiles.hi;
     g.whole = true;
-    g.begin = 0;
+    g.begin = g.slot = 0;
     g.units = 1;
 }
+// the prefix's
+__device__ __forceinline__ void attn_part(const AttentionArgs& a, const AttentionEntry& e, uint32_t parts, AttnSegment& g) {
+    const smelt_serving::AttentionJob j = smelt_serving::attention_job(a, e, parts, blockIdx.x);
+    g.row_tile = j.row_tile;
+    g.kv_head = j.kv_head;
+    g.tiles = AttentionTiles{0, e.front_tiles};
+    g.first = smelt_serving::attention_part_start(e.front_tiles, parts, j.part);
+    g.last = smelt_serving::attention_part_start(e.front_tiles, parts, j.part + 1);
+    g.whole = parts == 1;
+    g.begin = 0;
+    g.units = 1;
+    g.slot = (j.row_tile * a.kv_heads + j.kv_head) * parts + j.part;
+}
 
-// the slot of the part of a segment that workgroup w leaves
+// where the part of a segment goes that is not the whole of it
 __device__ __forceinline__ float* attn_piece(const AttentionArgs& a, const AttnSegment& g, uint32_t dim) {
-    const uint32_t slot = a.by_segment ? blockIdx.x + g.row_tile * a.kv_heads + g.kv_head : 2 * blockIdx.x + (g.first == g.tiles.lo ? 1u : 0u);
-    return a.pieces + (size_t)slot * smelt_serving::piece_floats(a.row_tile, dim);
+    return a.pieces + (size_t)g.slot * smelt_serving::piece_floats(a.row_tile, dim);
 }
 // the last workgroup that has a part of a segment
 __device__ __forceinline__ uint32_t attn_last(const AttentionSplit& split, const AttnSegment& g) {
@@ -192,15 +214,21 @@ __device__ __forceinline__ smelt_serving::AttentionCut attn_cut(const AttentionA
     return {attn_last(split, g), g.kv_head, e.first_token, row0, left < a.row_tile ? left : a.row_tile, {0, 0, 0}};
 }
 // kOwnKeys, kPrefix: ends a row (r within its tile) of a segment that begins here
-__device__ __forceinline__ void attn_end_row(float* end, const AttentionArgs& a, const AttentionSplit& split, const AttnSegment& g, uint32_t r, float max, float sum) {
-    const uint32_t parts = g.whole ? 1u : attn_last(split, g) - blockIdx.x + 1u;
-    const uint32_t slot = a.by_segment ? blockIdx.x + g.row_tile * a.kv_heads + g.kv_head : 2 * blockIdx.x + 1;
-    *reinterpret_cast<smelt_serving::AttentionRowEnd*>(end) = smelt_serving::AttentionRowEnd{max, sum, slot, parts << 8 | r};
+__device__ __forceinline__ void attn_end_row(float* end, const AttentionArgs& a, const AttnWork& work, const AttnSegment& g, uint32_t r, float max, float sum) {
+    const uint32_t parts = g.whole ? 1u : (work.parts ? work.parts : attn_last(work.split, g) - blockIdx.x + 1u);
+    *reinterpret_cast<smelt_serving::AttentionRowEnd*>(end) = smelt_serving::AttentionRowEnd{max, sum, g.slot, parts << 8 | r};
 }
 
-// the sequence of a token row: offsets is ascending, tokens before offsets[sequences] belong to one
+// The sequence of a lane's token row: offsets is ascending, tokens before offsets[sequences] belong to one.  The wave takes 64 of the
+// offsets at once (the steps of a search in memory are a load's latency each, six or more of them).
 __device__ __forceinline__ uint32_t sequence_of(const AttentionArgs& a, uint32_t token) {
-    uint32_t lo = 0, hi = a.sequences;   // offsets[lo] <= token < offsets[hi]
+    const uint32_t step = (a.sequences + kWave - 1) / kWave, mine = (threadIdx.x % kWave) * step;
+    const uint32_t sample = mine < a.sequences ? smelt_serving::clamp_count(a.offsets[mine], a.tokens) : ~0u;
+    uint32_t lo = 0;
+#pragma unroll
+    for (uint32_t bit = kWave / 2; bit; bit /= 2) lo = (uint32_t)__shfl((int)sample, (int)(lo + bit)) <= token ? lo + bit : lo;
+    lo *= step;
+    uint32_t hi = lo + step < a.sequences ? lo + step : a.sequences;   // offsets[lo] <= token < offsets[hi]
 #pragma unroll 1
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
@@ -429,14 +457,15 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
     attn_note_cut(a, {});
     if (work.entry == ~0u) return;
     uint32_t unit = work.at, index = work.entry, base = work.base;
-    const uint32_t unit_end = smelt_serving::attention_start(work.split, blockIdx.x + 1);
+    const uint32_t unit_end = work.parts ? unit + 1 : smelt_serving::attention_start(work.split, blockIdx.x + 1);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, quarter = lane >> 4, col = lane & 15;
     const AttnScale scale = attn_scale(a);
 #pragma unroll 1
     while (unit < unit_end) {
         const AttentionEntry e = attn_entry(a, index);
         AttnSegment g;
-        if (!attn_segment(a, e, base, unit, unit_end, g)) { base = g.begin; ++index; continue; }
+        if (work.parts) attn_part(a, e, work.parts, g);
+        else if (!attn_segment(a, e, base, unit, unit_end, g)) { base = g.begin; ++index; continue; }
         unit += g.units;
         if (g.first >= g.last) continue;                 // (only some of its lead)
         const uint32_t row0 = g.row_tile * R;
@@ -604,7 +633,7 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
             }
             const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
             float* dst = attn_whole_row(a, token, head, D);
-            if (a.part != smelt_serving::kWholeSequences && begins && d == 0) attn_end_row(dst + D, a, work.split, g, r, top, sum);
+            if (a.part != smelt_serving::kWholeSequences && begins && d == 0) attn_end_row(dst + D, a, work, g, r, top, sum);
             if (!g.whole) {
                 *reinterpret_cast<float4_t*>(piece + 2 * R + r * D + d) = y;
                 if (d == 0) { piece[r] = top; piece[R + r] = sum; }
@@ -649,7 +678,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
     attn_note_cut(a, {});
     if (work.entry == ~0u) return;
     uint32_t unit = work.at, index = work.entry, base = work.base;
-    const uint32_t unit_end = work.split.whole ? unit + 1 : smelt_serving::attention_start(work.split, blockIdx.x + 1);
+    const uint32_t unit_end = work.parts || work.split.whole ? unit + 1 : smelt_serving::attention_start(work.split, blockIdx.x + 1);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, half = lane >> 5;
     const AttnScale scale = attn_scale(a);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem);
@@ -669,7 +698,8 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
     while (unit < unit_end) {
         const AttentionEntry e = attn_entry(a, index);
         AttnSegment g;
-        if (work.split.whole) attn_whole_segment(a, e, unit - base, g);
+        if (work.parts) attn_part(a, e, work.parts, g);
+        else if (work.split.whole) attn_whole_segment(a, e, unit - base, g);
         else if (!attn_segment(a, e, base, unit, unit_end, g)) { base = g.begin; ++index; continue; }
         unit += g.units;
         if (g.first >= g.last) continue;                 // (only some of its lead)
@@ -851,7 +881,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                 float* whole = attn_whole_row(a, row.token, head, D);
                 float* dst = g.whole ? whole : piece + 2 * R + r * D;
                 if (half == 0) {
-                    if (a.part != smelt_serving::kWholeSequences && begins) attn_end_row(whole + D, a, work.split, g, r, acc.m, l);
+                    if (a.part != smelt_serving::kWholeSequences && begins) attn_end_row(whole + D, a, work, g, r, acc.m, l);
                     if (!g.whole) { piece[r] = acc.m; piece[R + r] = l; }
                 }
 #pragma unroll
@@ -884,7 +914,7 @@ __device__ __forceinline__ void attn_join_pieces(AttnJoin& j, const AttentionArg
 #pragma unroll
         for (uint32_t k = 0; k < U; ++k) {
             const uint32_t w = base + k < parts ? base + k : parts - 1;
-            uint32_t slot = a.by_segment ? first + w : (w ? 2 * (first / 2 + w) : first);
+            uint32_t slot = a.part == smelt_serving::kPrefix ? first + w : (w ? 2 * (first / 2 + w) : first);
             slot = slot < a.slots ? slot : a.slots - 1;
             const float* piece = a.pieces + (size_t)slot * smelt_serving::piece_floats(a.row_tile, D);
             m[k] = piece[r];
@@ -941,7 +971,7 @@ __device__ __forceinline__ void attn_combine_shared(const smelt_serving::Attenti
         auto join = [&](const AttentionArgs& x, const smelt_serving::AttentionRowEnd& end, float4_t y) {
             // (offsets that do not ascend leave rows without a segment: whatever is there stays within the slots)
             uint32_t parts = end.parts_row >> 8, r = end.parts_row & 255u;
-            parts = parts < x.workgroups ? parts : x.workgroups;
+            parts = parts < x.slots ? parts : x.slots;
             r = r < x.row_tile ? r : x.row_tile - 1;
             if (parts <= 1) attn_join(j, end.max, end.sum, y, x.scale_log2);
             else attn_join_pieces<D>(j, x, end.piece < x.slots ? end.piece : 0u, parts, r, d, x.scale_log2);

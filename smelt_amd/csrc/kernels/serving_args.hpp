@@ -45,7 +45,8 @@ struct RopeArgs {
 // once.  An entry is cut into segments: a tile of `row_tile` rows (token, head of the group) of one kv head, against the key
 // tiles that any of its rows sees.  The workgroups take equal runs of the resulting units: `lead` units for beginning a segment,
 // then one for each of its key tiles; row tiles ascending, within them the kv heads, within them the units.  Where there are enough
-// segments for that, each workgroup takes one.
+// segments for that, each workgroup takes one.  The prefix's segments are all alike and are cut into equal parts instead, a workgroup
+// each.
 constexpr uint32_t kKeyTile = 32;
 enum AttentionPart : uint32_t { kWholeSequences = 0, kOwnKeys = 1, kPrefix = 2 };
 
@@ -80,10 +81,10 @@ struct AttentionArgs {
     uint32_t pages = 0, page_shift = 0, pages_per_sequence = 0, prefix_pages = 0;
     uint32_t window = 0, q_stride = 0, workgroups = 0, part = 0;
     uint32_t row_tile = 0;
-    uint32_t by_segment = 0;       // a part's slot: workgroup + segment (one entry), or else 2 * workgroup, + 1 for one that begins its segment
     uint32_t slots = 0;
+    uint32_t rounds = 1;           // kPrefix: workgroups times rounds that a launch has at most
     uint32_t lead = 0;             // what beginning a segment costs, in key tiles
-    uint32_t least_units = 1;      // a workgroup takes at least this many units
+    uint32_t least_units = 1;      // a workgroup takes at least this many units (kPrefix: key tiles)
     uint32_t whole_from = ~0u;     // segments from which on each workgroup takes one
     float scale_log2 = 0;          // |scale| * log2(e)
     uint32_t flip_q = 0;           // 0x80008000 for a negative scale
@@ -181,6 +182,43 @@ SMELT_HD uint32_t attention_start(const AttentionSplit& s, uint32_t w) { return 
 SMELT_HD uint32_t attention_owner(const AttentionSplit& s, uint32_t u) {
     const uint32_t border = s.longer * (s.each + 1);
     return u < border ? u / (s.each + 1) : s.longer + (u - border) / s.each;
+}
+
+// The parts that the prefix's segments are cut into (0: no rows): one, two ... workgroups for every place the machine has, whichever
+// ends first, `lead` being what a part costs besides its key tiles.
+SMELT_HD uint32_t attention_parts(const AttentionArgs& a, const AttentionEntry& e) {
+    const uint32_t segments = attention_segments(a, e), tiles = e.front_tiles;
+    if (segments == 0) return 0;
+    uint32_t most = a.slots / segments, best = 1, cost = ~0u;
+    const uint32_t long_enough = tiles / a.least_units;
+    most = most < long_enough ? most : long_enough;
+    for (uint32_t r = 1; r <= a.rounds; ++r) {
+        uint32_t parts = r * a.workgroups / segments;
+        parts = parts < most ? parts : most;
+        parts = parts ? parts : 1u;
+        const uint32_t took = (segments * parts + a.workgroups - 1) / a.workgroups * ((tiles + parts - 1) / parts + a.lead);
+        if (took < cost) { cost = took; best = parts; }
+    }
+    return best;
+}
+// What workgroup w of a prefix launch takes.  The row tiles that read the same keys are neighbours, and neighbours are the workgroups that
+// share a second-level cache (every eighth).
+struct AttentionJob { uint32_t row_tile, kv_head, part; bool some; };
+SMELT_HD AttentionJob attention_job(const AttentionArgs& a, const AttentionEntry& e, uint32_t parts, uint32_t w) {
+    const uint32_t jobs = attention_segments(a, e) * parts, each = (jobs + 7) / 8, job = (w % 8) * each + w / 8;
+    AttentionJob j{0, 0, 0, w / 8 < each && job < jobs};
+    if (j.some) {
+        j.row_tile = job % e.row_tiles;
+        const uint32_t rest = job / e.row_tiles;
+        j.kv_head = rest / parts;
+        j.part = rest - j.kv_head * parts;
+    }
+    return j;
+}
+// first key tile of part p
+SMELT_HD uint32_t attention_part_start(uint32_t tiles, uint32_t parts, uint32_t p) {
+    const uint32_t each = tiles / parts, longer = tiles - each * parts;
+    return p * each + (p < longer ? p : longer);
 }
 
 // ---- verification of drafted tokens ----------------------------------------------------------------------------------

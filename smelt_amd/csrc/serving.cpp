@@ -14,6 +14,7 @@ using namespace smelt_serving;
 namespace {
 
 constexpr uint32_t kSegmentLead = 4;     // what beginning a segment of rows and keys costs, in key tiles
+constexpr uint32_t kPartLead = 8;        // ... a workgroup with a part of the prefix
 
 // "_d256" at `at`: the number behind the letters, and the position behind it
 bool number_after(const std::string& s, const char* letters, size_t* at, uint32_t* out) {
@@ -282,34 +283,38 @@ int Planner::attention() {
     const bool stream = rows <= (uint64_t)32 * a.sequences;
     const uint32_t tile_rows = dim == 256 ? 128 : 256;
     auto row_tile = [&](uint64_t of, uint64_t over) { return of <= 16 * over ? 16u : (of <= 32 * over ? 32u : tile_rows); };
-    // The parts of cut segments live in the context's workspace, a workgroup leaving two at most (of its first and its last segment).
-    // Against the prefix, whose tiles are large, the parts are counted along workgroups and segments instead, where that is fewer.
+    // The parts of cut segments live in the context's workspace, a workgroup leaving two at most (of its first and its last segment),
+    // or one of the prefix's.
     const size_t row_region = (size_t)a.tokens * a.heads * (dim + 4) * 4;
     auto piece_bytes = [&](uint32_t r) { return (size_t)piece_floats(r, dim) * 4; };
+    auto segments = [&](const AttentionArgs& x) { return ((rows + x.row_tile - 1) / x.row_tile + (x.part == kPrefix ? 0 : x.sequences)) * x.kv_heads; };   // there can be
     auto lay_out = [&](AttentionArgs& x, uint32_t r, size_t room) {
         x.row_tile = r;
-        x.lead = kSegmentLead;
-        x.least_units = x.lead + (r <= 32 ? 4 : 8);       // a key tile for each of four waves; stages to keep under way
         // workgroups that the register file holds
         const uint32_t per_cu = r == 16 ? (dim == 256 ? 2 : (dim == 128 ? 3 : 4)) : (r == 32 && dim != 256 ? 2 : 1);
-        const size_t most = (size_t)dev.compute_units * per_cu, slots = room / piece_bytes(r);
-        const uint64_t segments = (rows + r - 1) / r * a.kv_heads;
-        x.by_segment = x.part == kPrefix && segments < most && segments < slots / 2;
-        x.workgroups = (uint32_t)std::min<size_t>(most, x.by_segment ? slots - segments : slots / 2);
-        x.slots = x.by_segment ? x.workgroups + (uint32_t)segments : 2 * x.workgroups;
+        const size_t most = (size_t)dev.compute_units * per_cu;
+        x.slots = (uint32_t)std::min<size_t>(2 * most, room / piece_bytes(r));
+        if (x.part == kPrefix) {
+            x.workgroups = (uint32_t)most;
+            x.lead = kPartLead;
+            x.least_units = 8;
+            x.rounds = segments(x) > most / 4 ? 2 : 1;
+        } else {
+            x.workgroups = (uint32_t)std::min<size_t>(most, x.slots / 2);
+            x.lead = kSegmentLead;
+            x.least_units = x.lead + (r <= 32 ? 4 : 8);   // a key tile for each of four waves; stages to keep under way
+        }
         // a segment each from three quarters of the workgroups on: no parts to write and join
         x.whole_from = r <= 32 ? ~0u : std::max(1u, dev.compute_units * 3 / 4);
     };
     char* ws = static_cast<char*>(dev.workspace);
     auto main_step = [&](const AttentionArgs& x) {
         const uint32_t r = x.row_tile;
-        if (r <= 32) {
-            step(r == 16 ? 0 : 1, x, x.workgroups, 1, 1, 256, (size_t)4 * r * (dim + 4) * 4 + 2 * 4 * r * 4);
-            return;
-        }
-        // as many as there can be segments
-        const uint64_t most = (((uint64_t)x.tokens * x.group + r - 1) / r + (x.part == kPrefix ? 0 : x.sequences)) * x.kv_heads;
-        step(2, x, (uint32_t)std::max<uint64_t>(x.workgroups, std::min<uint64_t>(most, 0x7FFFFFFFull)), 1, 1, dim == 256 ? 256 : 512, (size_t)4 * (dim == 256 ? 1 : 2) * 2 * 32 * dim * 2);
+        // (as many as there can be segments, where each may take one)
+        uint64_t grid = x.part == kPrefix ? (std::max<uint64_t>(segments(x), x.workgroups * x.rounds) + 7) / 8 * 8 : (r <= 32 ? x.workgroups : std::max<uint64_t>(segments(x), x.workgroups));
+        grid = std::min<uint64_t>(grid, 0x7FFFFFF8ull);
+        if (r <= 32) step(r == 16 ? 0 : 1, x, (uint32_t)grid, 1, 1, 256, (size_t)4 * r * (dim + 4) * 4 + 2 * 4 * r * 4);
+        else step(2, x, (uint32_t)grid, 1, 1, dim == 256 ? 256 : 512, (size_t)4 * (dim == 256 ? 1 : 2) * 2 * 32 * dim * 2);
     };
     // units are counted in 32 bits
     const uint64_t key_tiles = ((uint64_t)a.pages_per_sequence + a.prefix_pages) * page / kKeyTile + 2;
@@ -326,7 +331,7 @@ int Planner::attention() {
         lay_out(both.own, own_rows, room / 2);
         const size_t own_bytes = both.own.slots * piece_bytes(own_rows);
         lay_out(both.front, front_rows, room - own_bytes);
-        if (both.own.workgroups && both.front.workgroups) {
+        if (both.own.workgroups) {
             both.own.pieces = reinterpret_cast<float*>(ws + 2 * row_region);
             both.front.pieces = reinterpret_cast<float*>(ws + 2 * row_region + own_bytes);
             main_step(both.front);
