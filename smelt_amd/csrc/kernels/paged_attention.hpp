@@ -365,6 +365,15 @@ __device__ __forceinline__ void attn_hide(float16_t& s, int32_t key0, const Attn
     }
 }
 
+// The outputs stay in the matrix instructions' own registers on both ways around the rare rescaling (the compiler would copy all of them
+// to vector registers in front of it and back, for every tile).
+template <int D>
+__device__ __forceinline__ void attn_keep(AttnAcc<D>& acc) {
+    if constexpr (D < 256) return;       // (two waves a SIMD: they have no others)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) asm volatile("" : "+a"(acc.o[j]));
+}
+
 template <int D, int NS>
 __device__ __forceinline__ void attn_softmax(const AttnScale& c, AttnAcc<D>& acc, float16_t* s) {
     float top = s[0][0];
@@ -373,6 +382,7 @@ __device__ __forceinline__ void attn_softmax(const AttnScale& c, AttnAcc<D>& acc
 #pragma unroll
         for (int i = 0; i < 16; i += 2) top = __builtin_fmaxf(__builtin_fmaxf(top, s[n][i]), s[n][i + 1]);
     top = attn_halves_max(top);
+    attn_keep(acc);
     if (__any(top > acc.m + c.slack)) {      // also the first finite score: the maximum starts at -inf
         const float m = __builtin_fmaxf(acc.m, top);
         const float f = m == -__builtin_inff() ? 1.0f : attn_exp2((acc.m - m) * c.c);
@@ -382,6 +392,7 @@ __device__ __forceinline__ void attn_softmax(const AttnScale& c, AttnAcc<D>& acc
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc.o[j][i] *= f;
         acc.m = m;
+        attn_keep(acc);
     }
     const float shift = acc.m == -__builtin_inff() ? 0.0f : -acc.m * c.c;
     float sum[2] = {0.0f, 0.0f};
@@ -661,9 +672,10 @@ constexpr int kAttnBuffers = 4;
 template <int D>
 __device__ __forceinline__ uint32_t attn_v_turn(uint32_t row) { return D == 64 ? (row >> 1) & 1u : row & 3u; }
 
-// 16 bytes a lane from base + offset to LDS at `lds` + 16 * lane; counts as a vector load, in order
+// 16 bytes a lane from base + offset to LDS at `lds` + 16 * lane; counts as a vector load, in order.  (Five wait states: the compiler
+// does not see that a vector load reads the base, which a vector instruction may have written just before.)
 __device__ __forceinline__ void attn_load_lds(uint64_t base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 // waits until at most N of the wave's vector loads are under way
 template <int N>
@@ -674,12 +686,17 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr uint32_t R = 32 * WAVES, kHalf = 16 * D * 2, kTile = 4 * kHalf, kStage = NS * kTile;      // bytes: K halves, V halves
     constexpr int P = D / (8 * WAVES), kPerHalf = D / 32;       // loads of a wave a tile; wave loads a half
+    constexpr bool kOneHalf = WAVES >= 2 * kPerHalf;            // a wave's loads are all of one half's keys or values
+    constexpr uint32_t kRowShift = D == 256 ? 9 : (D == 128 ? 8 : 7);   // bytes of a V row
+    constexpr uint32_t kAllThere = (1u << 2 * NS) - 1;
     const AttnWork work = find_work(a, blockIdx.x);
     attn_note_cut(a, {});
     if (work.entry == ~0u) return;
     uint32_t unit = work.at, index = work.entry, base = work.base;
     const uint32_t unit_end = work.parts || work.split.whole ? unit + 1 : smelt_serving::attention_start(work.split, blockIdx.x + 1);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, half = lane >> 5;
+    const uint32_t my_half = (wave / kPerHalf) & 1u;
+    const bool my_value = wave / (2 * kPerHalf) != 0;
     const AttnScale scale = attn_scale(a);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem);
     // the lane's place in each of the wave's loads: piece `at` of a half, K [dim / 8][key][8] or V [key][dim]
@@ -724,6 +741,12 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
             const AttnRun u = attn_run(a, e, run, row0, 32, &b, 1);
             const uint32_t stages = (last - first + NS - 1) / NS;
 
+            // stages whose every key all of the wave's rows see (so the run does not end inside one either)
+            const uint32_t seen_lo = u.all_lo > 0 ? ((uint32_t)u.all_lo + 31) / 32 : 0u, seen_hi = u.all_hi > 0 ? (uint32_t)u.all_hi / 32 : 0u;
+            const uint32_t plain_lo = __builtin_amdgcn_readfirstlane(seen_lo > first ? (seen_lo - first + NS - 1) / NS : 0u);
+            const uint32_t plain_hi = __builtin_amdgcn_readfirstlane(seen_hi > first ? (seen_hi - first) / NS : 0u);
+            const uint32_t plain_n = plain_hi > plain_lo ? plain_hi - plain_lo : 0u;
+
             // pages of a stage's half tiles; past the run's part its last tile once more, so that every stage is the same number of loads
             struct Pages { uint32_t id[NS][2]; };
             auto pages_of = [&](uint32_t stage) {
@@ -740,35 +763,41 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                     }
                 return p;
             };
-            uint32_t pages_known = 0;                     // four bits a buffer, two a tile: the halves are on pages of the pool's
+            uint32_t there = 0;                           // 2 NS bits a stage, the last fetched lowest: the half tiles that are there, on pages of the pool's
             auto fetch = [&](uint32_t stage, const Pages& pages) {
-                const uint32_t buffer = stage % kAttnBuffers;
-                pages_known &= ~(15u << (4 * buffer));
+                const uint32_t to = lds0 + (stage % kAttnBuffers) * kStage;
+                there <<= 2 * NS;
 #pragma unroll
                 for (int n = 0; n < NS; ++n) {
                     uint32_t tile = first + stage * NS + n;
-                    tile = tile < last ? tile : last - 1;
+                    const bool some = tile < last;
+                    tile = some ? tile : last - 1;
                     uint64_t at[2];
                     uint32_t off[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const bool known = pages.id[n][h] < a.pages;
-                        pages_known |= known ? 1u << (4 * buffer + 2 * n + h) : 0u;
+                        there |= known && some ? 1u << (2 * n + h) : 0u;
                         at[h] = (uint64_t)(known ? pages.id[n][h] : 0u) * page_bytes;
                         off[h] = (tile * 32 + 16 * h) & page_mask;
                     }
+                    if constexpr (kOneHalf) {
+                        at[0] = my_half ? at[1] : at[0];
+                        off[0] = my_half ? off[1] : off[0];
+                    }
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
-                        const uint32_t q = p * WAVES + wave, region = q / kPerHalf, h = region & 1;
-                        const uint64_t page = h ? at[1] : at[0];
-                        const uint32_t o = h ? off[1] : off[0];
-                        const uint64_t from = region < 2 ? k_base + page + o * 16 : v_base + page + o * (D * 2);
-                        attn_load_lds(from, offset[p], lds0 + buffer * kStage + n * kTile + q * 1024);
+                        const int h = kOneHalf ? 0 : (p * WAVES / kPerHalf) & 1;
+                        const bool value = P == 1 ? my_value : p >= P / 2;
+                        attn_load_lds((value ? v_base : k_base) + at[h] + (off[h] << (value ? kRowShift : 4u)), offset[p], to + n * kTile + (p * WAVES + wave) * 1024);
                     }
                 }
             };
 #pragma unroll 1
-            for (uint32_t s = 0; s < kAttnBuffers - 1 && s < stages; ++s) fetch(s, pages_of(s));
+            for (uint32_t s = 0; s < kAttnBuffers - 1; ++s) {
+                if (s < stages) fetch(s, pages_of(s));
+                else there <<= 2 * NS;
+            }
             Pages pages = pages_of(kAttnBuffers - 1);
             // (the compiler counts its own loads alone: from here on only stages are under way)
             if (run == 0 || e.front_tiles == 0) attn_wait_loads<0>();
@@ -780,58 +809,46 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                 if (stage + kAttnBuffers - 1 <= stages) attn_wait_loads<(kAttnBuffers - 2) * P * NS>();
                 else attn_wait_loads<0>();
                 __syncthreads();
-                // what the wave's rows see of the stage, and what there is of it (a tile past the part's end: nothing)
-                bool seen = false, edge[NS], ragged = false;
-                uint32_t known[NS];
-                int32_t key0[NS];
-#pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    const uint32_t tile = first + stage * NS + n;
-                    const bool some = tile < last;
-                    key0[n] = (int32_t)tile * (int32_t)smelt_serving::kKeyTile;
-                    known[n] = some ? (pages_known >> (4 * buffer + 2 * n)) & 3u : 0u;
-                    seen = seen || (some && attn_seen(u, key0[n]));
-                    edge[n] = known[n] != 3u || attn_masked(u, key0[n]);
-                    ragged = ragged || known[n] != 3u || (uint32_t)key0[n] + 32 > len;
-                }
+                const uint32_t known = (there >> (2 * NS * (kAttnBuffers - 2))) & kAllThere;
+                const bool plain = stage - plain_lo < plain_n && known == kAllThere;
                 const unsigned char* st = smem + buffer * kStage;
-                if (ragged) {
+                if (known != kAllThere || (first + (stage + 1) * NS) * smelt_serving::kKeyTile > len) {
                     // Values of keys behind the run's end, or on a page that is none of the pool's, are whatever memory holds: zero them,
                     // since a zero probability does not silence an infinity or a NaN.
 #pragma unroll 1
                     for (int n = 0; n < NS; ++n) {
+                        const uint32_t key0 = (first + stage * NS + n) * smelt_serving::kKeyTile;
                         uint4_t* v = reinterpret_cast<uint4_t*>(smem + buffer * kStage + n * kTile + 2 * kHalf);
                         for (uint32_t p = threadIdx.x; p < 4 * D; p += 64 * WAVES) {
                             const uint32_t key = p / (D / 8);
-                            if ((uint32_t)key0[n] + key >= len || !((known[n] >> (key / 16)) & 1u)) v[p] = uint4_t{0, 0, 0, 0};
+                            if (key0 + key >= len || !((known >> (2 * n + key / 16)) & 1u)) v[p] = uint4_t{0, 0, 0, 0};
                         }
                     }
                     __syncthreads();
                 }
                 // operands are read well before the products that take them: K of a tile while the one before is multiplied, V before the softmax
                 float16_t s[NS];
-                if (seen) {
-                    uint4_t kf[2][D / 16];
-                    auto load_k = [&](int n) {
-                        const uint4_t* kl = reinterpret_cast<const uint4_t*>(st + n * kTile + k_lane);
+                uint4_t kf[2][D / 16];
+                auto load_k = [&](int n) {
+                    const uint4_t* kl = reinterpret_cast<const uint4_t*>(st + n * kTile + k_lane);
 #pragma unroll
-                        for (int d = 0; d < D / 16; ++d) kf[n & 1][d] = kl[d * 32];
-                    };
-                    load_k(0);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int d = 0; d < D / 16; ++d) kf[n & 1][d] = kl[d * 32];
+                };
+                load_k(0);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int n = 0; n < NS; ++n) {
-                        if (n + 1 < NS) { load_k(n + 1); __builtin_amdgcn_sched_barrier(0); }
-                        s[n] = attn_mfma<ActT>(kf[n & 1][0], qf[0], float16_t{});
+                for (int n = 0; n < NS; ++n) {
+                    if (n + 1 < NS) { load_k(n + 1); __builtin_amdgcn_sched_barrier(0); }
+                    s[n] = attn_mfma<ActT>(kf[n & 1][0], qf[0], float16_t{});
 #pragma unroll
-                        for (int d = 1; d < D / 16; ++d) s[n] = attn_mfma<ActT>(kf[n & 1][d], qf[d], s[n]);
-                    }
+                    for (int d = 1; d < D / 16; ++d) s[n] = attn_mfma<ActT>(kf[n & 1][d], qf[d], s[n]);
                 }
                 if (stage + kAttnBuffers - 1 < stages) {
                     fetch(stage + kAttnBuffers - 1, pages);
                     pages = pages_of(stage + kAttnBuffers);
+                } else {
+                    there <<= 2 * NS;
                 }
-                if (!seen) continue;
                 uint4_t vf[NS][2][D / 32];
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
@@ -846,9 +863,10 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                             vf[n][h][j] = uint4_t{lo.x, lo.y, hi.x, hi.y};
                         }
                 __builtin_amdgcn_sched_barrier(0);
+                if (!plain) {
 #pragma unroll
-                for (int n = 0; n < NS; ++n)
-                    if (edge[n]) attn_hide(s[n], key0[n], b, known[n]);
+                    for (int n = 0; n < NS; ++n) attn_hide(s[n], (int32_t)((first + stage * NS + n) * smelt_serving::kKeyTile), b, known >> (2 * n));
+                }
                 attn_softmax<D, NS>(scale, acc, s);
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
