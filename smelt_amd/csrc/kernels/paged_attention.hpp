@@ -78,6 +78,7 @@ struct AttnWork {
     uint32_t base;           // units (segments where each workgroup takes one) before that entry
     uint32_t at;             // the unit (segment)
     uint32_t parts;          // kPrefix: of each segment
+    smelt_serving::AttentionJob job;
 };
 
 // Each wave looks for itself (no barrier), an entry a lane: once through the entries for their total, then for the wanted one.
@@ -87,10 +88,12 @@ __device__ __forceinline__ AttnWork find_work(const AttentionArgs& a, uint32_t g
     w.entry = ~0u;
     w.base = w.at = w.parts = 0;
     w.split = AttentionSplit{0, 0, 0, 0, false};
+    w.job = smelt_serving::AttentionJob{0, 0, 0, false};
     if (a.part == smelt_serving::kPrefix) {
         const AttentionEntry e = attn_entry(a, 0);
         w.parts = smelt_serving::attention_parts(a, e);
-        if (smelt_serving::attention_job(a, e, w.parts, group).some) w.entry = 0;
+        w.job = smelt_serving::attention_job(a, e, w.parts, group);
+        if (w.job.some) w.entry = 0;
         return w;
     }
     uint32_t mine[2] = {0, 0}, before[2] = {0, 0}, all[2] = {0, 0};      // units and segments: the lane's entry, the entries before it in the round, the round's
@@ -184,13 +187,15 @@ __device__ __forceinline__ void attn_whole_segment(const AttentionArgs& a, const
     g.units = 1;
 }
 // the prefix's
-__device__ __forceinline__ void attn_part(const AttentionArgs& a, const AttentionEntry& e, uint32_t parts, AttnSegment& g) {
-    const smelt_serving::AttentionJob j = smelt_serving::attention_job(a, e, parts, blockIdx.x);
+__device__ __forceinline__ void attn_part(const AttentionArgs& a, const AttentionEntry& e, const AttnWork& work, AttnSegment& g) {
+    const smelt_serving::AttentionJob& j = work.job;
+    const uint32_t parts = work.parts;
     g.row_tile = j.row_tile;
     g.kv_head = j.kv_head;
     g.tiles = AttentionTiles{0, e.front_tiles};
-    g.first = smelt_serving::attention_part_start(e.front_tiles, parts, j.part);
-    g.last = smelt_serving::attention_part_start(e.front_tiles, parts, j.part + 1);
+    const uint32_t each = e.front_tiles / parts, longer = e.front_tiles - each * parts;
+    g.first = j.part * each + (j.part < longer ? j.part : longer);
+    g.last = g.first + each + (j.part < longer ? 1u : 0u);
     g.whole = parts == 1;
     g.begin = 0;
     g.units = 1;
@@ -475,7 +480,7 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
     while (unit < unit_end) {
         const AttentionEntry e = attn_entry(a, index);
         AttnSegment g;
-        if (work.parts) attn_part(a, e, work.parts, g);
+        if (work.parts) attn_part(a, e, work, g);
         else if (!attn_segment(a, e, base, unit, unit_end, g)) { base = g.begin; ++index; continue; }
         unit += g.units;
         if (g.first >= g.last) continue;                 // (only some of its lead)
@@ -715,7 +720,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
     while (unit < unit_end) {
         const AttentionEntry e = attn_entry(a, index);
         AttnSegment g;
-        if (work.parts) attn_part(a, e, work.parts, g);
+        if (work.parts) attn_part(a, e, work, g);
         else if (work.split.whole) attn_whole_segment(a, e, unit - base, g);
         else if (!attn_segment(a, e, base, unit, unit_end, g)) { base = g.begin; ++index; continue; }
         unit += g.units;

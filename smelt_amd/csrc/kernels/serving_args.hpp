@@ -215,11 +215,6 @@ SMELT_HD AttentionJob attention_job(const AttentionArgs& a, const AttentionEntry
     }
     return j;
 }
-// first key tile of part p
-SMELT_HD uint32_t attention_part_start(uint32_t tiles, uint32_t parts, uint32_t p) {
-    const uint32_t each = tiles / parts, longer = tiles - each * parts;
-    return p * each + (p < longer ? p : longer);
-}
 
 // ---- verification of drafted tokens ----------------------------------------------------------------------------------
 // A row's logits are cut into `runs` runs of `span` (a multiple of kVerifyStep), each the work of one wave; the launches leave a
