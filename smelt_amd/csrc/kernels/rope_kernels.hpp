@@ -66,90 +66,116 @@ __device__ __forceinline__ size_t rope_at(const RopeArgs& a, const RopeRows& r, 
     return base + ((((size_t)(d >> 3) << a.page_shift) + off) << 3) + (d & 7u);
 }
 
-// one unit of a rotated head: a pair of 16-byte pieces (half), one piece (interleaved), or a copied piece;
-// without VEC one pair of values, or one copied value
-template <class ActT, bool VEC, int TARGET>
-__device__ __forceinline__ void rope_unit(const RopeArgs& a, const RopeRows& r, const float2* cs, uint32_t token, int32_t slot, uint32_t head, uint32_t unit) {
-    const uint16_t* src = r.src + (size_t)token * r.src_stride + (size_t)head * a.dim;
-    auto at = [&](uint32_t d) { return r.dst + rope_at<TARGET>(a, r, token, slot, head, d); };
-    if (VEC) {
-        const uint32_t rotated = a.interleaved ? a.rot / 8 : a.rot / 16;
-        if (TARGET == kToValues || unit >= rotated) {
-            const uint32_t d = TARGET == kToValues ? unit * 8 : a.rot + (unit - rotated) * 8;
-            *reinterpret_cast<uint4_t*>(at(d)) = *reinterpret_cast<const uint4_t*>(src + d);
-            return;
-        }
-        const uint32_t d = unit * 8;
-        float x[8], y[8];
-        unpack8<ActT>(*reinterpret_cast<const uint4_t*>(src + d), x);
-        if (a.interleaved) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 w = cs[d / 2 + k];
-                y[2 * k] = x[2 * k] * w.x - x[2 * k + 1] * w.y;
-                y[2 * k + 1] = x[2 * k + 1] * w.x + x[2 * k] * w.y;
-            }
-            *reinterpret_cast<uint4_t*>(at(d)) = pack8<ActT>(y);
-        } else {
-            const uint32_t d2 = d + a.rot / 2;
-            float x2[8], y2[8];
-            unpack8<ActT>(*reinterpret_cast<const uint4_t*>(src + d2), x2);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float2 w = cs[d + k];
-                y[k] = x[k] * w.x - x2[k] * w.y;
-                y2[k] = x2[k] * w.x + x[k] * w.y;
-            }
-            *reinterpret_cast<uint4_t*>(at(d)) = pack8<ActT>(y);
-            *reinterpret_cast<uint4_t*>(at(d2)) = pack8<ActT>(y2);
-        }
+// What a unit of a token's work is: a pair of 16-byte pieces of a rotated head (half), one piece (interleaved), or a copied piece;
+// without VEC one pair of values, or one copied value.
+struct RopeUnit {
+    int target;
+    uint32_t tok, head, d, d2;      // d2: the pair's other piece or value, d where there is none
+    bool copied;
+};
+
+// unit i of a workgroup's: the tokens' q units, then the k units, then the v units
+template <bool VEC, bool APPEND>
+__device__ __forceinline__ RopeUnit rope_unit(const RopeArgs& a, uint32_t shift, uint32_t i) {
+    RopeUnit x;
+    x.target = kToRows;
+    uint32_t u;
+    if (!APPEND || i < a.q.units << shift) {
+        x.tok = fast_div(i, a.q.units, a.q_units_inv);
+        u = i - x.tok * a.q.units;
     } else {
-        const uint32_t pairs = a.rot / 2;
-        if (TARGET == kToValues || unit >= pairs) {
-            const uint32_t d = TARGET == kToValues ? unit : a.rot + (unit - pairs);
-            *at(d) = src[d];
-            return;
+        i -= a.q.units << shift;
+        x.target = kToKeys;
+        x.tok = i & ((1u << shift) - 1u);
+        u = i >> shift;
+        if (u >= a.k.units) {
+            i -= a.k.units << shift;
+            x.target = kToValues;
+            x.tok = fast_div(i, a.v.units, a.v_units_inv);
+            u = i - x.tok * a.v.units;
         }
-        const uint32_t d0 = a.interleaved ? 2 * unit : unit, d1 = a.interleaved ? 2 * unit + 1 : unit + pairs;
-        const float x0 = ActT::widen(src[d0]), x1 = ActT::widen(src[d1]);
-        const float2 w = cs[unit];
-        *at(d0) = ActT::narrow(x0 * w.x - x1 * w.y);
-        *at(d1) = ActT::narrow(x1 * w.x + x0 * w.y);
     }
+    const bool value = x.target == kToValues;
+    x.head = value ? fast_div(u, a.per_copy, a.per_copy_inv) : fast_div(u, a.per_head, a.per_head_inv);
+    const uint32_t unit = u - x.head * (value ? a.per_copy : a.per_head);
+    const uint32_t one = VEC ? 8u : 1u, rotated = VEC ? (a.interleaved ? a.rot / 8 : a.rot / 16) : a.rot / 2;
+    x.copied = value || unit >= rotated;
+    if (x.copied) x.d = x.d2 = value ? unit * one : a.rot + (unit - rotated) * one;
+    else if (!a.interleaved) { x.d = unit * one; x.d2 = x.d + a.rot / 2; }
+    else if (VEC) x.d = x.d2 = unit * 8;
+    else { x.d = 2 * unit; x.d2 = x.d + 1; }
+    return x;
+}
+// (the fields are chosen one by one: a chosen set of rows would have to lie in memory)
+template <bool APPEND>
+__device__ __forceinline__ const uint16_t* rope_src(const RopeArgs& a, const RopeUnit& x, uint32_t first) {
+    const uint16_t* src = a.q.src;
+    uint32_t stride = a.q.src_stride;
+    if (APPEND && x.target == kToKeys) { src = a.k.src; stride = a.k.src_stride; }
+    if (APPEND && x.target == kToValues) { src = a.v.src; stride = a.v.src_stride; }
+    return src + (size_t)(first + x.tok) * stride + (size_t)x.head * a.dim;
+}
+template <bool APPEND>
+__device__ __forceinline__ uint16_t* rope_dst(const RopeArgs& a, const RopeUnit& x, uint32_t first, int32_t slot, uint32_t d) {
+    if (APPEND && x.target == kToKeys) return a.k.dst + rope_at<kToKeys>(a, a.k, first + x.tok, slot, x.head, d);
+    if (APPEND && x.target == kToValues) return a.v.dst + rope_at<kToValues>(a, a.v, first + x.tok, slot, x.head, d);
+    return a.q.dst + rope_at<kToRows>(a, a.q, first + x.tok, 0, x.head, d);
 }
 
-// One workgroup per `tokens_per_group` tokens; its threads walk the tokens' units.
+// One workgroup per `tokens_per_group` (a power of two) tokens.  Its threads take units in turn: along the rows that are stored as they
+// are read, and token after token for keys, since the 16-byte pieces that neighbouring tokens put into a key page lie side by side.
 template <class ActT, bool VEC, bool APPEND>
 __device__ __forceinline__ void rope_body(const RopeArgs& a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const uint32_t pairs = a.rot / 2;
     float2* cs = reinterpret_cast<float2*>(smem);
-    const uint32_t first = blockIdx.x * a.tokens_per_group;
+    int32_t* slots = reinterpret_cast<int32_t*>(cs + a.tokens_per_group * pairs);
+    const uint32_t first = blockIdx.x * a.tokens_per_group, shift = 31 - __builtin_clz(a.tokens_per_group);
     const uint32_t count = a.tokens - first < a.tokens_per_group ? a.tokens - first : a.tokens_per_group;
+    if (APPEND && threadIdx.x < count) slots[threadIdx.x] = a.slots[first + threadIdx.x];
     rope_angles(a, first, count, cs);
     __syncthreads();
-    const uint32_t pairs = a.rot / 2;
-    for (uint32_t i = threadIdx.x; i < count * a.per_token; i += blockDim.x) {
-        const uint32_t tok = fast_div(i, a.per_token, a.per_token_inv);
-        uint32_t u = i - tok * a.per_token;
-        const uint32_t token = first + tok;
-        const float2* w = cs + tok * pairs;
-        if (!APPEND || u < a.q.units) {
-            const uint32_t head = fast_div(u, a.per_head, a.per_head_inv);
-            rope_unit<ActT, VEC, kToRows>(a, a.q, w, token, 0, head, u - head * a.per_head);
-            continue;
+    for (uint32_t i = threadIdx.x; i < a.per_token << shift; i += blockDim.x) {
+        const RopeUnit x = rope_unit<VEC, APPEND>(a, shift, i);
+        if (x.tok >= count) continue;
+        int32_t slot = 0;
+        if (APPEND && x.target != kToRows) {
+            slot = slots[x.tok];
+            if (slot < 0 || ((uint32_t)slot >> a.page_shift) >= a.pages) continue;      // nowhere to go
         }
-        if (APPEND) {
-            u -= a.q.units;
-            const int32_t slot = a.slots[token];
-            if (slot < 0 || ((uint32_t)slot >> a.page_shift) >= a.pages) continue;   // nowhere to go
-            if (u < a.k.units) {
-                const uint32_t head = fast_div(u, a.per_head, a.per_head_inv);
-                rope_unit<ActT, VEC, kToKeys>(a, a.k, w, token, slot, head, u - head * a.per_head);
+        const uint16_t* src = rope_src<APPEND>(a, x, first);
+        uint16_t* to = rope_dst<APPEND>(a, x, first, slot, x.d);
+        const float2* w = cs + x.tok * pairs;
+        if constexpr (VEC) {
+            const uint4_t in = *reinterpret_cast<const uint4_t*>(src + x.d);
+            if (x.copied) { *reinterpret_cast<uint4_t*>(to) = in; continue; }
+            float v[8], y[8];
+            unpack8<ActT>(in, v);
+            if (a.interleaved) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 z = w[x.d / 2 + q];
+                    y[2 * q] = v[2 * q] * z.x - v[2 * q + 1] * z.y;
+                    y[2 * q + 1] = v[2 * q + 1] * z.x + v[2 * q] * z.y;
+                }
             } else {
-                u -= a.k.units;
-                const uint32_t head = fast_div(u, a.per_copy, a.per_copy_inv);
-                rope_unit<ActT, VEC, kToValues>(a, a.v, w, token, slot, head, u - head * a.per_copy);
+                float v2[8], y2[8];
+                unpack8<ActT>(*reinterpret_cast<const uint4_t*>(src + x.d2), v2);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float2 z = w[x.d + q];
+                    y[q] = v[q] * z.x - v2[q] * z.y;
+                    y2[q] = v2[q] * z.x + v[q] * z.y;
+                }
+                *reinterpret_cast<uint4_t*>(rope_dst<APPEND>(a, x, first, slot, x.d2)) = pack8<ActT>(y2);
             }
+            *reinterpret_cast<uint4_t*>(to) = pack8<ActT>(y);
+        } else {
+            if (x.copied) { *to = src[x.d]; continue; }
+            const float x0 = ActT::widen(src[x.d]), x1 = ActT::widen(src[x.d2]);
+            const float2 z = w[a.interleaved ? x.d / 2 : x.d];
+            *to = ActT::narrow(x0 * z.x - x1 * z.y);
+            *rope_dst<APPEND>(a, x, first, slot, x.d2) = ActT::narrow(x1 * z.x + x0 * z.y);
         }
     }
 }

@@ -224,15 +224,18 @@ int Planner::rope() {
     a.v.units = kv_heads * a.per_copy;
     a.per_token = a.q.units + a.k.units + a.v.units;
     if (a.per_token > kRopeMaxPerToken) return bad("one token has more than " + std::to_string(kRopeMaxPerToken) + " pieces to move");
-    a.per_token_inv = reciprocal(a.per_token);
     a.per_head_inv = reciprocal(a.per_head);
+    a.q_units_inv = reciprocal(a.q.units);
+    a.v_units_inv = reciprocal(a.v.units);
     a.per_copy_inv = reciprocal(a.per_copy);
-    // A workgroup takes several tokens when there are enough for every compute unit all the same, so that its threads all have an
-    // angle to form; n * d of the reciprocal division stays below 2^32 (65535 pieces a token, 65536 units a workgroup)
+    // A workgroup takes several tokens when there are enough for every compute unit all the same, so that its threads all have an angle
+    // to form, and so that what neighbouring tokens put into a key page (16 bytes each) makes whole cache lines; n * d of the
+    // reciprocal division stays below 2^32 (65535 pieces a token, 65536 units a workgroup)
     uint32_t group = 1;
-    while (group < 8 && half && (group * 2) * half <= kRopeThreads && a.tokens / (group * 2) >= 4 * dev.compute_units && (uint64_t)group * 2 * a.per_token <= 65536) group *= 2;
+    const uint32_t most = append ? 16 : 8, angles = append ? 4 * kRopeThreads : kRopeThreads, least = (append ? 2 : 4) * dev.compute_units;
+    while (group < most && half && (group * 2) * half <= angles && a.tokens / (group * 2) >= least && (uint64_t)group * 2 * a.per_token <= 65536) group *= 2;
     a.tokens_per_group = group;
-    step(vec ? 0 : 1, a, (a.tokens + group - 1) / group, 1, 1, kRopeThreads, (size_t)group * half * 8 + 16);
+    step(vec ? 0 : 1, a, (a.tokens + group - 1) / group, 1, 1, kRopeThreads, (size_t)group * half * 8 + 64);
     return 0;
 }
 
