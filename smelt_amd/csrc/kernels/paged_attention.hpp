@@ -430,6 +430,44 @@ __device__ __forceinline__ void attn_clear(AttnAcc<D>& acc) {
         for (int i = 0; i < 16; ++i) acc.o[j][i] = 0.0f;
 }
 
+// Values are multiplied with a zero probability where one of a tile's rows does not see a key and another does, and a zero does not silence
+// an infinity or a NaN.  Rows that came out as NaN are therefore formed once more at a segment's end, key after key (maxima and sums
+// are right: hidden scores are taken out before those).  Slow, and outside of the key loops, which looking for such values cost a fifth
+// of their time.
+//
+// Calls use(whether a row of the given bounds sees it, the first 8 dims of its K, its V row) for the keys of the workgroup's part of a
+// segment.
+template <int D, class Bounds, class Use>
+__device__ __forceinline__ void attn_each_key(const AttentionArgs& a, const AttentionEntry& e, const AttnSegment& g, Bounds bounds, Use use) {
+#pragma unroll 1
+    for (int run = 0; run < 2; ++run) {
+        const uint32_t len = run ? e.own : e.front, tile0 = run ? e.front_tiles : 0u;
+        const uint32_t first = (g.first > tile0 ? g.first - tile0 : 0u) * smelt_serving::kKeyTile;
+        uint32_t last = (g.last > tile0 ? g.last - tile0 : 0u) * smelt_serving::kKeyTile;
+        last = last < len ? last : len;
+        const scalar_table table = as_scalar(run ? a.page_table + (size_t)e.sequence * a.pages_per_sequence : a.prefix_table);
+        const AttnBounds b = bounds(run ? (int32_t)e.prefix : 0, (int32_t)len);
+#pragma unroll 1
+        for (uint32_t key = first; key < last; ++key) {
+            const uint32_t page = (uint32_t)table[__builtin_amdgcn_readfirstlane(key >> a.page_shift)], off = key & ((1u << a.page_shift) - 1u);
+            if (page >= a.pages) continue;
+            const size_t at = (((size_t)page * a.kv_heads + g.kv_head) * D) << a.page_shift;
+            use((int32_t)key >= b.lo && (int32_t)key < b.hi, a.k_cache + at + off * 8, a.v_cache + at + off * D);
+        }
+    }
+}
+// products of eight pairs of 16-bit values, added up
+template <class ActT>
+__device__ __forceinline__ float attn_dot8(uint4_t x, uint4_t y) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sum = __builtin_fmaf(ActT::widen((uint16_t)(x[i] & 0xFFFFu)), ActT::widen((uint16_t)(y[i] & 0xFFFFu)), sum);
+        sum = __builtin_fmaf(ActT::widen((uint16_t)(x[i] >> 16)), ActT::widen((uint16_t)(y[i] >> 16)), sum);
+    }
+    return sum;
+}
+
 // maximum and sum over a lane's row of the streaming kernel: lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float attn_quarters_max(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
@@ -453,6 +491,7 @@ template <int D, int RT>
 struct AttnShared {
     float o[4][16 * RT][D + 4];      // (four floats of padding: neighbouring rows' 16-byte stores lie on different banks)
     float m[4][16 * RT], l[4][16 * RT];
+    int32_t position[16 * RT];
 };
 
 // Few rows a sequence (decoding, drafted tokens): bound by the cache's bytes.  A workgroup takes a run of units and works
@@ -615,7 +654,7 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const float sum = attn_quarters_sum(l[t]);
-            if (lane < 16) { sh.m[wave][16 * t + lane] = m[t]; sh.l[wave][16 * t + lane] = sum; }
+            if (lane < 16) { sh.m[wave][16 * t + lane] = m[t]; sh.l[wave][16 * t + lane] = sum; sh.position[16 * t + lane] = row[t].position; }
             if (row[t].live) {
 #pragma unroll
                 for (int c = 0; c < VC; ++c)
@@ -648,6 +687,21 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
                 sum += f * sh.l[w][r];
             }
             const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
+            if (y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w) {
+                const uint16_t* q = a.q + (size_t)token * a.q_stride + (size_t)head * D;
+                const float shift = top == -__builtin_inff() ? 0.0f : -top * scale.c;
+                y = float4_t{0, 0, 0, 0};
+                attn_each_key<D>(a, e, g, [&](int32_t base, int32_t len) { return attn_bounds(a, AttnRow{true, token, 0, sh.position[r]}, base, len); },
+                                 [&](bool sees, const uint16_t* k, const uint16_t* v) {
+                    float dot = 0.0f;
+#pragma unroll 1
+                    for (uint32_t n = 0; n < D; ++n)
+                        dot = __builtin_fmaf(ActT::widen((uint16_t)(q[n] ^ (uint16_t)a.flip_q)), ActT::widen(k[((n / 8) << (a.page_shift + 3)) + n % 8]), dot);
+                    const float p = attn_exp2(__builtin_fmaf(dot, scale.c, shift));
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) y[n] = sees ? __builtin_fmaf(p, ActT::widen(v[d + n]), y[n]) : y[n];
+                });
+            }
             float* dst = attn_whole_row(a, token, head, D);
             if (a.part != smelt_serving::kWholeSequences && begins && d == 0) attn_end_row(dst + D, a, work, g, r, top, sum);
             if (!g.whole) {
@@ -680,6 +734,8 @@ __device__ __forceinline__ uint32_t attn_v_turn(uint32_t row) { return D == 64 ?
 // 16 bytes a lane from base + offset to LDS at `lds` + 16 * lane; counts as a vector load, in order.  (Five wait states: the compiler
 // does not see that a vector load reads the base, which a vector instruction may have written just before.)
 __device__ __forceinline__ void attn_load_lds(uint64_t base, uint32_t offset, uint32_t lds) {
+    base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base);
+    lds = __builtin_amdgcn_readfirstlane(lds);
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 // waits until at most N of the wave's vector loads are under way
@@ -889,6 +945,34 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
         if (begins && !g.whole) attn_note_cut(a, attn_cut(a, e, work.split, g));
         float* piece = attn_piece(a, g, D);
         const float l = attn_halves_sum(acc.l);
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) nan = nan || acc.o[j][i] != acc.o[j][i];
+        if (__any(nan && row.live)) {
+            const float m = acc.m, shift = m == -__builtin_inff() ? 0.0f : -m * scale.c;
+            attn_clear<D>(acc);
+            acc.m = m;
+            attn_each_key<D>(a, e, g, [&](int32_t base, int32_t len) { return attn_bounds(a, row, base, len); },
+                             [&](bool sees, const uint16_t* k, const uint16_t* v) {
+                float dot = 0.0f;
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n) dot += attn_dot8<ActT>(qf[n], *reinterpret_cast<const uint4_t*>(k + ((2 * n + half) << (a.page_shift + 3))));
+                const float p = attn_exp2(__builtin_fmaf(attn_halves_sum(dot), scale.c, shift));
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const uint2_t w = *reinterpret_cast<const uint2_t*>(v + 32 * j + 2 * i + 4 * half);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const float x = ActT::widen((uint16_t)(w[n / 2] >> (16 * (n & 1))));
+                            acc.o[j][i + n] = sees ? __builtin_fmaf(p, x, acc.o[j][i + n]) : acc.o[j][i + n];
+                        }
+                    }
+            });
+        }
         if (row.live) {
             const uint32_t r = wave * 32 + (lane & 31), head = g.kv_head * a.group + row.head;
             if (g.whole && a.part == smelt_serving::kWholeSequences) {

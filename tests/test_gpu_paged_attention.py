@@ -244,3 +244,50 @@ def test_attention_is_refused_where_a_slot_is_short(ctx):
     with pytest.raises(rt.SmeltHipError, match="aligned"):
         go(tokens=1, sequences=1, out=B(7, 2))
     ctx.wait()
+
+
+def bad_values(case, at, dims):
+    """Infinities and NaN among the values of sequence s's own keys at[s], in `dims`."""
+    bad = np.array([0x7C00, 0x7E00, 0xFC00] if case.dtype == fx.F16 else [0x7F80, 0x7FC0, 0xFF80], np.uint16)
+    for s, keys in enumerate(at):
+        for n, j in enumerate(keys):
+            page, off = case.table[s, j // case.page], j % case.page
+            for m, d in enumerate(dims):
+                case.vb[page, :, off, d] = bad[(n + m) % 3]
+
+
+def check_where_finite(case, got):
+    """The result is not finite exactly where the rows that see such a value say so, and right everywhere else."""
+    y, reach, sharp, count = case.want()
+    live = int(case.offsets[-1])
+    tol = sr.attention_tolerance(y, np.where(np.isfinite(reach), reach, 0.0), sharp, count, case.dim, case.dtype)[:live]
+    g, y = sr.wide(got[:live], case.dtype).reshape(y[:live].shape), y[:live]
+    assert np.array_equal(np.isnan(g), np.isnan(y))
+    assert np.array_equal(np.isposinf(g), np.isposinf(y)) and np.array_equal(np.isneginf(g), np.isneginf(y))
+    ok = np.isfinite(y)
+    assert ok.any() and not ok.all()
+    assert np.all(np.abs(g - y)[ok] <= tol[ok])
+
+
+# rows a sequence: one row tile of 16, of 32, the kernel for many rows; the prefix apart, and with the own keys
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,prefix", [([3, 2], 0), ([8, 5], 0), ([70, 33], 0), ([3, 2], 45), ([70, 33], 45)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_infinities_in_keys_that_only_some_rows_see(ctx, dtype, dim, n, prefix, window):
+    c = Case(ctx, dtype, n, [n[0] + 90, n[1] + 31], 8, 2, dim, 16, prefix=prefix, window=window, poison=False)
+    ends = [int(c.lens[s]) for s in range(2)]
+    bad_values(c, [[ends[0] - 1, ends[0] - 2], [ends[1] - 1]], [0, 5, dim - 1])
+    table = c.load()
+    c.ctx.interpret_decode(table)
+    c.ctx.wait()
+    check_where_finite(c, c.result())
+
+
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 40])
+def test_infinities_in_keys_before_every_rows_window(ctx, dtype, dim, n):
+    c = Case(ctx, dtype, [n], [n + 100], 4, 2, dim, 64, window=9, poison=False)
+    bad_values(c, [[100 - 9, 100 - 12]], range(dim))       # (the first row's position is 100: it sees keys 92 on)
+    c.run()
