@@ -456,18 +456,6 @@ __device__ __forceinline__ void attn_each_key(const AttentionArgs& a, const Atte
         }
     }
 }
-// products of eight pairs of 16-bit values, added up
-template <class ActT>
-__device__ __forceinline__ float attn_dot8(uint4_t x, uint4_t y) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        sum = __builtin_fmaf(ActT::widen((uint16_t)(x[i] & 0xFFFFu)), ActT::widen((uint16_t)(y[i] & 0xFFFFu)), sum);
-        sum = __builtin_fmaf(ActT::widen((uint16_t)(x[i] >> 16)), ActT::widen((uint16_t)(y[i] >> 16)), sum);
-    }
-    return sum;
-}
-
 // maximum and sum over a lane's row of the streaming kernel: lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float attn_quarters_max(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
@@ -687,7 +675,7 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
                 sum += f * sh.l[w][r];
             }
             const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
-            if (y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w) {
+            if (__builtin_expect(y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w, 0)) {
                 const uint16_t* q = a.q + (size_t)token * a.q_stride + (size_t)head * D;
                 const float shift = top == -__builtin_inff() ? 0.0f : -top * scale.c;
                 y = float4_t{0, 0, 0, 0};
@@ -950,29 +938,9 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) nan = nan || acc.o[j][i] != acc.o[j][i];
-        if (__any(nan && row.live)) {
-            const float m = acc.m, shift = m == -__builtin_inff() ? 0.0f : -m * scale.c;
-            attn_clear<D>(acc);
-            acc.m = m;
-            attn_each_key<D>(a, e, g, [&](int32_t base, int32_t len) { return attn_bounds(a, row, base, len); },
-                             [&](bool sees, const uint16_t* k, const uint16_t* v) {
-                float dot = 0.0f;
-#pragma unroll
-                for (int n = 0; n < D / 16; ++n) dot += attn_dot8<ActT>(qf[n], *reinterpret_cast<const uint4_t*>(k + ((2 * n + half) << (a.page_shift + 3))));
-                const float p = attn_exp2(__builtin_fmaf(attn_halves_sum(dot), scale.c, shift));
-#pragma unroll
-                for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const uint2_t w = *reinterpret_cast<const uint2_t*>(v + 32 * j + 2 * i + 4 * half);
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const float x = ActT::widen((uint16_t)(w[n / 2] >> (16 * (n & 1))));
-                            acc.o[j][i + n] = sees ? __builtin_fmaf(p, x, acc.o[j][i + n]) : acc.o[j][i + n];
-                        }
-                    }
-            });
-        }
+        const unsigned long long nans = __ballot(nan && row.live);
+        const uint32_t again = (uint32_t)nans | (uint32_t)(nans >> 32);          // rows
+        const bool done = !((again >> (lane & 31)) & 1u);
         if (row.live) {
             const uint32_t r = wave * 32 + (lane & 31), head = g.kv_head * a.group + row.head;
             if (g.whole && a.part == smelt_serving::kWholeSequences) {
@@ -982,7 +950,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                 for (int j = 0; j < D / 32; ++j)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<uint2_t*>(out + 32 * j + 2 * i) = uint2_t{attn_pack2<ActT>(acc.o[j][i] * inv, acc.o[j][i + 1] * inv),
+                        if (done) *reinterpret_cast<uint2_t*>(out + 32 * j + 2 * i) = uint2_t{attn_pack2<ActT>(acc.o[j][i] * inv, acc.o[j][i + 1] * inv),
                                                                                    attn_pack2<ActT>(acc.o[j][i + 2] * inv, acc.o[j][i + 3] * inv)};
             } else {
                 float* whole = attn_whole_row(a, row.token, head, D);
@@ -995,7 +963,37 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                 for (int j = 0; j < D / 32; ++j)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<float4_t*>(dst + 4 * half + 32 * j + 2 * i) = float4_t{acc.o[j][i], acc.o[j][i + 1], acc.o[j][i + 2], acc.o[j][i + 3]};
+                        if (done) *reinterpret_cast<float4_t*>(dst + 4 * half + 32 * j + 2 * i) = float4_t{acc.o[j][i], acc.o[j][i + 1], acc.o[j][i + 2], acc.o[j][i + 3]};
+            }
+        }
+        // (a lane takes D / 64 values of one row after the other here)
+        for (uint32_t set = again; set; set &= set - 1) {
+            constexpr int E = D / 64;
+            const int from = __builtin_ctz(set);
+            const uint32_t d = lane * E, r = wave * 32 + from, token = __builtin_amdgcn_readlane(row.token, from), head = g.kv_head * a.group + __builtin_amdgcn_readlane(row.head, from);
+            const int32_t position = __builtin_amdgcn_readlane(row.position, from);
+            const float m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, acc.m), from)), sum = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), from));
+            const float shift = m == -__builtin_inff() ? 0.0f : -m * scale.c;
+            float q[E], y[E];
+#pragma unroll
+            for (int n = 0; n < E; ++n) { q[n] = ActT::widen((uint16_t)(a.q[(size_t)token * a.q_stride + (size_t)head * D + d + n] ^ (uint16_t)a.flip_q)); y[n] = 0.0f; }
+            attn_each_key<D>(a, e, g, [&](int32_t base, int32_t len) { return attn_bounds(a, AttnRow{true, token, 0, position}, base, len); },
+                             [&](bool sees, const uint16_t* k, const uint16_t* v) {
+                float dot = 0.0f;
+#pragma unroll
+                for (int n = 0; n < E; ++n) dot = __builtin_fmaf(q[n], ActT::widen(k[((d / 8) << (a.page_shift + 3)) + d % 8 + n]), dot);
+#pragma unroll
+                for (int off = 32; off > 0; off >>= 1) dot += __shfl_xor(dot, off);
+                const float p = attn_exp2(__builtin_fmaf(dot, scale.c, shift));
+#pragma unroll
+                for (int n = 0; n < E; ++n) y[n] = sees ? __builtin_fmaf(p, ActT::widen(v[d + n]), y[n]) : y[n];
+            });
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int n = 0; n < E; ++n) {
+                if (g.whole && a.part == smelt_serving::kWholeSequences) a.out[((size_t)token * a.heads + head) * D + d + n] = ActT::narrow(y[n] * inv);
+                else if (g.whole) attn_whole_row(a, token, head, D)[d + n] = y[n];
+                else piece[2 * R + r * D + d + n] = y[n];
             }
         }
     }
