@@ -694,7 +694,7 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
             if (a.part != smelt_serving::kWholeSequences && begins && d == 0) attn_end_row(dst + D, a, work, g, r, top, sum);
             if (!g.whole) {
                 *reinterpret_cast<float4_t*>(piece + 2 * R + r * D + d) = y;
-                if (d == 0) { piece[r] = top; piece[R + r] = sum; }
+                if (d == 0) *reinterpret_cast<float2*>(piece + 2 * r) = float2{top, sum};
             } else if (a.part != smelt_serving::kWholeSequences) {
                 *reinterpret_cast<float4_t*>(dst + d) = y;
             } else {
@@ -957,7 +957,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                 float* dst = g.whole ? whole : piece + 2 * R + r * D;
                 if (half == 0) {
                     if (a.part != smelt_serving::kWholeSequences && begins) attn_end_row(whole + D, a, work, g, r, acc.m, l);
-                    if (!g.whole) { piece[r] = acc.m; piece[R + r] = l; }
+                    if (!g.whole) *reinterpret_cast<float2*>(piece + 2 * r) = float2{acc.m, l};
                 }
 #pragma unroll
                 for (int j = 0; j < D / 32; ++j)
@@ -1011,10 +1011,10 @@ __device__ __forceinline__ void attn_join(AttnJoin& j, float m, float l, float4_
 // row r of `parts` parts of a segment, the first in slot `first`
 template <int D>
 __device__ __forceinline__ void attn_join_pieces(AttnJoin& j, const AttentionArgs& a, uint32_t first, uint32_t parts, uint32_t r, uint32_t d, float c) {
-    constexpr uint32_t U = 8;      // parts whose loads are under way together
+    constexpr uint32_t U = 12;     // parts whose loads are under way together
 #pragma unroll 1
     for (uint32_t base = 0; base < parts; base += U) {
-        float m[U], l[U];
+        float2 ml[U];
         float4_t y[U];
 #pragma unroll
         for (uint32_t k = 0; k < U; ++k) {
@@ -1022,13 +1022,12 @@ __device__ __forceinline__ void attn_join_pieces(AttnJoin& j, const AttentionArg
             uint32_t slot = a.part == smelt_serving::kPrefix ? first + w : (w ? 2 * (first / 2 + w) : first);
             slot = slot < a.slots ? slot : a.slots - 1;
             const float* piece = a.pieces + (size_t)slot * smelt_serving::piece_floats(a.row_tile, D);
-            m[k] = piece[r];
-            l[k] = piece[a.row_tile + r];
+            ml[k] = *reinterpret_cast<const float2*>(piece + 2 * r);
             y[k] = *reinterpret_cast<const float4_t*>(piece + 2 * a.row_tile + r * D + d);
         }
 #pragma unroll
         for (uint32_t k = 0; k < U; ++k)
-            if (base + k < parts) attn_join(j, m[k], l[k], y[k], c);
+            if (base + k < parts) attn_join(j, ml[k].x, ml[k].y, y[k], c);
     }
 }
 template <class ActT>

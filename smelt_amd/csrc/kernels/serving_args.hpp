@@ -74,7 +74,7 @@ struct AttentionArgs {
     const int32_t* prefix_table = nullptr;
     const int32_t* prefix_len = nullptr;
     uint16_t* out = nullptr;
-    float* pieces = nullptr;       // slots of [row_tile] max, [row_tile] sum, [row_tile][dim]
+    float* pieces = nullptr;       // slots of [row_tile] (max, sum), [row_tile][dim]
     float* rows = nullptr;         // not kWholeSequences: [dim] and an AttentionRowEnd a (token, head)
     AttentionCut* cuts = nullptr;  // kWholeSequences: one a workgroup
     uint32_t tokens = 0, sequences = 0, heads = 0, kv_heads = 0, group = 0;
