@@ -267,8 +267,9 @@ int smelt_emit_paged_kv_append(smelt_emitter *e, const SmeltRope *rope, const Sm
  * kv_lens[s] keys of its own, its new tokens' included, on the pages of page_table[s][pages_per_sequence].  prefix_table (at most
  * prefix_pages pages) and prefix_len (one int32) name a prefix that stands before every sequence's own keys; it is read once for
  * all of them when they have few rows each.  The last row of a sequence is the newest key's; a row sees the keys up to its
- * own and, with window > 0, only the last `window` of them.  A row that sees nothing is zero.  Lengths are cut to what the tables
- * hold; keys on a page outside the pool are not seen. */
+ * own and, with window > 0, only the last `window` of them.  A row that sees nothing is zero.  Infinities and NaN among keys and values
+ * that a row does not see leave it as it is (rows of such a tile are formed a second time, slowly).  Lengths are cut to what the tables
+ * hold; keys on a page outside the pool are not seen.  Offsets that do not ascend leave rows unspecified, and nothing else touched. */
 int smelt_emit_paged_attention(smelt_emitter *e, const SmeltPagedCache *cache, SmeltBinding q,
                                SmeltBinding page_table, SmeltBinding kv_lens, SmeltBinding offsets,
                                SmeltBinding output, const SmeltBinding *prefix_table,

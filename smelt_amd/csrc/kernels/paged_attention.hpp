@@ -299,7 +299,6 @@ __device__ __forceinline__ AttnRun attn_run(const AttentionArgs& a, const Attent
     }
     return u;
 }
-__device__ __forceinline__ bool attn_seen(const AttnRun& u, int32_t key0) { return key0 < u.hi && key0 + (int32_t)smelt_serving::kKeyTile > u.lo; }
 __device__ __forceinline__ bool attn_masked(const AttnRun& u, int32_t key0) { return key0 + (int32_t)smelt_serving::kKeyTile > u.all_hi || key0 < u.all_lo; }
 
 // One wave's state: 32 rows.

@@ -108,6 +108,7 @@ struct Planner {
     const ServingDevice& dev;
     ServingPlan* plan;
     std::string* why;
+    bool too_wide = false;      // a launch of more threads than one can have
 
     int fail(int code, const std::string& m) { *why = m; return code; }
     int bad(const std::string& m) { return fail(SMELT_HIP_ERR_UNSUPPORTED_GEOMETRY, m); }
@@ -119,6 +120,7 @@ struct Planner {
     }
     template <class A> ServingStep& step(int kernel, const A& args, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t threads, size_t lds) {
         static_assert(sizeof(A) <= kServingArgBytes, "argument block");
+        too_wide = too_wide || (uint64_t)gx * threads > 0xFFFFFFFFull;
         ServingStep& s = plan->step[plan->steps++];
         s.kernel = kernel;
         s.grid[0] = gx; s.grid[1] = gy; s.grid[2] = gz;
@@ -259,6 +261,7 @@ int Planner::attention() {
     if ((uint64_t)a.tokens * a.heads > 0x7FFFFFFFull) return bad("more than 2^31 - 1 rows");
     if (a.q_stride < a.heads * dim) return bad("q's row stride is shorter than its heads");
     if (!std::isfinite(scale)) return bad("the scale must be finite");
+    if (a.window > 0x7FFFFFFFu) return bad("the window passes 2^31 - 1");
     // (a scale of zero weighs every key alike; the smallest normal number does the same and keeps a hidden key's -inf one)
     a.scale_log2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 1.2e-38f);
     a.flip_q = scale < 0.0f ? 0x80008000u : 0u;
@@ -315,7 +318,7 @@ int Planner::attention() {
         const uint32_t r = x.row_tile;
         // (as many as there can be segments, where each may take one)
         uint64_t grid = x.part == kPrefix ? (std::max<uint64_t>(segments(x), x.workgroups * x.rounds) + 7) / 8 * 8 : (r <= 32 ? x.workgroups : std::max<uint64_t>(segments(x), x.workgroups));
-        grid = std::min<uint64_t>(grid, 0x7FFFFFF8ull);
+        grid = std::min<uint64_t>(grid, 0xFFFFFFFFull);       // (refused for its threads)
         if (r <= 32) step(r == 16 ? 0 : 1, x, (uint32_t)grid, 1, 1, 256, (size_t)4 * r * (dim + 4) * 4 + 9 * r * 4);
         else step(2, x, (uint32_t)grid, 1, 1, dim == 256 ? 256 : 512, (size_t)4 * (dim == 256 ? 1 : 2) * 2 * 32 * dim * 2);
     };
@@ -410,16 +413,18 @@ int plan_serving(const ResolvedPipeline& r, const uint32_t* value, const Serving
     while (plan->operands < (int)r.kinds.size() && r.kinds[(size_t)plan->operands] == 'P') ++plan->operands;
     plan->steps = 0;
     Planner p{r, value, dev, plan, why};
+    int e;
     switch (r.family) {
         case kFamRope:
         case kFamPagedAppend:
-        case kFamPagedAppendQ: return p.rope();
+        case kFamPagedAppendQ: e = p.rope(); break;
         case kFamPagedAttention:
-        case kFamPagedAttentionShared: return p.attention();
+        case kFamPagedAttentionShared: e = p.attention(); break;
         case kFamVerifyDrafts:
-        case kFamVerifyDraftsGiven: return p.verify();
+        case kFamVerifyDraftsGiven: e = p.verify(); break;
         default: return p.bad("not a serving operator");
     }
+    return e == 0 && p.too_wide ? p.bad("one launch of more than 2^32 - 1 threads") : e;
 }
 
 }  // namespace smelt_host

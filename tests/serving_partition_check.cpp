@@ -48,6 +48,27 @@ uint64_t check_owners(uint32_t units, uint32_t workgroups, uint32_t least) {
     return 0;
 }
 
+// a prefix launch: parts of each segment, and what each of `grid` workgroups takes, {row_tile, kv_head, part} a workgroup that has some
+// (in order); returns how many have
+int check_jobs(const int32_t* offsets, int tokens, int sequences, int group, int kv_heads, int prefix, int row_tile, uint32_t workgroups, uint32_t rounds,
+               uint32_t slots, uint32_t least, uint32_t lead, uint32_t grid, uint32_t* parts, int32_t* jobs) {
+    AttentionArgs a;
+    const int32_t lens = 0;
+    a.offsets = offsets; a.kv_lens = &lens; a.sequences = sequences; a.tokens = tokens; a.group = group; a.kv_heads = kv_heads;
+    a.page_shift = 4; a.pages_per_sequence = 1; a.prefix_len = &prefix; a.prefix_pages = (prefix + 15) / 16; a.part = kPrefix;
+    a.row_tile = row_tile; a.workgroups = workgroups; a.rounds = rounds; a.slots = slots; a.least_units = least; a.lead = lead;
+    const AttentionEntry e = attention_entry(a, 0);
+    *parts = attention_parts(a, e);
+    int n = 0;
+    for (uint32_t w = 0; w < grid; ++w) {
+        const AttentionJob j = attention_job(a, e, *parts, w);
+        if (!j.some) continue;
+        jobs[3 * n] = j.row_tile; jobs[3 * n + 1] = j.kv_head; jobs[3 * n + 2] = j.part;
+        ++n;
+    }
+    return n;
+}
+
 uint32_t check_reciprocal(uint32_t d, uint32_t most) {
     const uint64_t inv = reciprocal(d);
     for (uint32_t n = 0; n <= most; ++n) {

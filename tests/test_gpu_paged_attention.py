@@ -291,3 +291,9 @@ def test_infinities_in_keys_before_every_rows_window(ctx, dtype, dim, n):
     c = Case(ctx, dtype, [n], [n + 100], 4, 2, dim, 64, window=9, poison=False)
     bad_values(c, [[100 - 9, 100 - 12]], range(dim))       # (the first row's position is 100: it sees keys 92 on)
     c.run()
+
+
+# the prefix's segments in six parts each (two for every compute unit), and whole (too short to be cut)
+@pytest.mark.parametrize("tokens,heads,kv_heads,prefix", [(600, 32, 4, 1700), (300, 64, 64, 200)])
+def test_a_prefix_behind_many_sequences(ctx, tokens, heads, kv_heads, prefix):
+    Case(ctx, fx.BF16, [1] * tokens, [1 + s % 5 for s in range(tokens)], heads, kv_heads, 64, 64, prefix=prefix, pad=3).run()

@@ -257,3 +257,39 @@ def test_every_unit_has_one_workgroup(partition):
 def test_reciprocal_division_is_exact(partition):
     for d in (1, 2, 3, 5, 7, 12, 17, 24, 96, 100, 255, 256, 1000, 4095, 4097, 65535):
         assert partition.check_reciprocal(d, min(2 ** 32 // max(d, 1) - 1, 70000)) == 0, d
+
+
+@pytest.mark.parametrize("tokens,group,kv_heads,prefix", [(64, 6, 4, 8192), (1, 1, 1, 1), (24, 4, 8, 2500), (1000, 8, 8, 300), (5, 3, 2, 40), (4096, 6, 4, 65), (700, 16, 1, 100000)])
+@pytest.mark.parametrize("row_tile", [16, 32, 128, 256])
+@pytest.mark.parametrize("slots", [0, 1, 100, 512])
+def test_every_part_of_the_prefix_has_one_workgroup(partition, tokens, group, kv_heads, prefix, row_tile, slots):
+    offsets, workgroups, least = np.array([0, tokens], np.int32), 256, 8
+    segments = -(-tokens * group // row_tile) * kv_heads
+    for rounds in (1, 2):
+        grid = -(-max(segments, workgroups * rounds) // 8) * 8          # what the launch has
+        parts, jobs = C.c_uint32(), np.zeros((grid, 3), np.int32)
+        n = partition.check_jobs(offsets.ctypes.data_as(C.POINTER(C.c_int32)), tokens, 1, group, kv_heads, prefix, row_tile, workgroups, rounds, slots, least, 8, grid,
+                                 C.byref(parts), jobs.ctypes.data_as(C.POINTER(C.c_int32)))
+        parts = parts.value
+        assert n == segments * parts and len({tuple(j) for j in jobs[:n].tolist()}) == n
+        assert jobs[:n].min() >= 0 and tuple(jobs[:n].max(0) + 1) == (segments // kv_heads, kv_heads, parts)
+        assert parts == 1 or (segments * parts <= min(slots, workgroups * rounds) and -(-prefix // 32) // parts >= least)
+
+
+def test_a_prefix_of_no_rows_has_no_parts(partition):
+    for offsets, prefix in (([0, 0], 100), ([0, 5], 0)):
+        parts, jobs = C.c_uint32(7), np.zeros((256, 3), np.int32)
+        assert partition.check_jobs(np.array(offsets, np.int32).ctypes.data_as(C.POINTER(C.c_int32)), 5, 1, 2, 2, prefix, 32, 256, 1, 512, 8, 8, 256, C.byref(parts),
+                                    jobs.ctypes.data_as(C.POINTER(C.c_int32))) == 0
+        assert parts.value == 0
+
+
+def test_launches_that_are_too_wide_are_refused():
+    em = cc.Emitter()
+    em.rope(B(1), B(2), B(3), B(4), tokens=30_000_000, heads=1, head_dim=256, rotary_dim=256)
+    refused(lambda: em.rope(B(1), B(2), B(3), B(4), tokens=60_000_000, heads=1, head_dim=256, rotary_dim=256), "threads")
+    # a workgroup for each of many segments that there can be, whatever the lengths are
+    att = dict(q=B(1), k_cache=B(2), v_cache=B(3), page_table=B(4), kv_lens=B(5), offsets=B(6), out=B(7), heads=64, kv_heads=64, head_dim=64, page_size=16, pages=100,
+               pages_per_sequence=1, scale=0.1)
+    em.paged_attention(**att, tokens=10_000_000, sequences=100)
+    refused(lambda: em.paged_attention(**att, tokens=33_000_000, sequences=200_000), "threads")
