@@ -31,7 +31,7 @@ struct RopeArgs {
     const int32_t* slots = nullptr;    // append: page * page_size + offset, negative = nowhere
     uint32_t tokens = 0, dim = 0, rot = 0, interleaved = 0;
     float amplitude = 1.0f;
-    uint32_t tokens_per_group = 1;     // tokens of one workgroup, a power of two up to 16
+    uint32_t tokens_per_group = 1;     // tokens of one workgroup, a power of two up to 4
     uint32_t per_token = 0, q_units_inv = 0, v_units_inv = 0;   // units of one token; ceil(2^32 / units) of its q and v
     uint32_t per_head = 0, per_head_inv = 0;     // units of one rotated head and ceil(2^32 / units)
     uint32_t per_copy = 0, per_copy_inv = 0;     // units of one head that is only copied (v)

@@ -11,6 +11,9 @@
 // exponentials: with a 248320-entry vocabulary neighbouring places in the running sum are 4e-6 apart and closer, and a 32-bit
 // exponential is already off by 6e-8 of each weight.  The first launch's 32-bit exponentials only meet the accept test, which they can
 // turn when u falls within about 1e-7 of the ratio.  Sums are added in a fixed order: the same inputs give the same tokens.
+// 64 sequences of 1 to 8 rows, 248320 logits: 105 us (254 MB, 50 us at a copy's rate): launch 1 takes 44 us (5.8 TB/s), 2 and 3 30 and
+// 22 us (the chosen rows' 64-bit exponentials: twenty 64-bit instructions a logit, about 14 us each), 4 takes 12.  One sequence: 26 us, four
+// launches of two or three dependent loads each.
 #pragma once
 #include "common.hpp"
 #include "serving_args.hpp"

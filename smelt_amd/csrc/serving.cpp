@@ -13,8 +13,11 @@ using namespace smelt_serving;
 
 namespace {
 
-constexpr uint32_t kSegmentLead = 4;     // what beginning a segment of rows and keys costs, in key tiles
-constexpr uint32_t kPartLead = 8;        // ... a workgroup with a part of the prefix
+// What beginning a segment of rows and keys costs, in key tiles (own keys of 64 sequences 38.8 / 37.5 / 37.6 us, one token 12.9 / 13.1 /
+// 14.0 us with 2 / 4 / 8) ...
+constexpr uint32_t kSegmentLead = 4;
+// ... and a workgroup's part of the prefix, whose 13 to 15 us besides the tiles' 1.5 weigh where a second round is looked at.
+constexpr uint32_t kPartLead = 8;
 
 // "_d256" at `at`: the number behind the letters, and the position behind it
 bool number_after(const std::string& s, const char* letters, size_t* at, uint32_t* out) {
@@ -230,12 +233,13 @@ int Planner::rope() {
     a.q_units_inv = reciprocal(a.q.units);
     a.v_units_inv = reciprocal(a.v.units);
     a.per_copy_inv = reciprocal(a.per_copy);
-    // A workgroup takes several tokens when there are enough for every compute unit all the same, so that its threads all have an angle
-    // to form, and so that what neighbouring tokens put into a key page (16 bytes each) makes whole cache lines; n * d of the
-    // reciprocal division stays below 2^32 (65535 pieces a token, 65536 units a workgroup)
+    // Append: a workgroup takes up to four tokens when there are enough for two workgroups a compute unit all the same, so that what
+    // neighbouring tokens put into a key page (16 bytes each) makes 64 contiguous bytes (8000 tokens of 8 heads of 128: 26.2 / 18.3 /
+    // 19.9 us at 1 / 4 / 8 tokens).  Rows: two, so that few heads keep the threads busy (8192 tokens of 32 heads of 128: 27.5 / 27.7 / 29.0
+    // us at 1 / 2 / 4).  n * d of the reciprocal division stays below 2^32 (65535 pieces a token, 65536 units a workgroup).
     uint32_t group = 1;
-    const uint32_t most = append ? 16 : 8, angles = append ? 4 * kRopeThreads : kRopeThreads, least = (append ? 2 : 4) * dev.compute_units;
-    while (group < most && half && (group * 2) * half <= angles && a.tokens / (group * 2) >= least && (uint64_t)group * 2 * a.per_token <= 65536) group *= 2;
+    const uint32_t most = append ? 4 : 2, least = (append ? 2 : 4) * dev.compute_units;
+    while (group < most && a.tokens / (group * 2) >= least && (uint64_t)group * 2 * a.per_token <= 65536) group *= 2;
     a.tokens_per_group = group;
     step(vec ? 0 : 1, a, (a.tokens + group - 1) / group, 1, 1, kRopeThreads, (size_t)group * half * 8 + 64);
     return 0;
@@ -285,6 +289,10 @@ int Planner::attention() {
 
     // The streaming kernel takes the sequences while they have few rows each (one tile of 16 or 32 rows on average), the prefix then
     // being read once against all rows; the tile kernel takes longer runs of rows, whose tiles read prefix and own keys alike.
+    // 64 sequences of 6 rows, heads of 256, a prefix of 8192: 86 us, with tiles of 32 rows 93, with the tile kernel for prefix and own keys
+    // 191.  24 sequences of 18 rows on average, heads of 128, a prefix of 2500: 67 us, with two tiles of 16 rows a sequence 69, with the
+    // tile kernel 60 (24 short sequences fill the machine once, and one launch is less than three; the lengths that would tell
+    // are not known here).
     const uint64_t rows = (uint64_t)a.tokens * a.group;
     const bool stream = rows <= (uint64_t)32 * a.sequences;
     const uint32_t tile_rows = dim == 256 ? 128 : 256;
@@ -303,14 +311,15 @@ int Planner::attention() {
         if (x.part == kPrefix) {
             x.workgroups = (uint32_t)most;
             x.lead = kPartLead;
-            x.least_units = 8;
+            x.least_units = 8;                // (24 sequences, a prefix of 2500: 68 / 67 / 72 us with parts of 3 / 8 / 16 key tiles at least)
             x.rounds = segments(x) > most / 4 ? 2 : 1;
         } else {
             x.workgroups = (uint32_t)std::min<size_t>(most, x.slots / 2);
             x.lead = kSegmentLead;
             x.least_units = x.lead + (r <= 32 ? 4 : 8);   // a key tile for each of four waves; stages to keep under way
         }
-        // a segment each from three quarters of the workgroups on: no parts to write and join
+        // a segment each from three quarters of the workgroups on: no parts to write and join (two prompt chunks of 1000 tokens behind
+        // 4000 keys, 240 segments: 137 us, in equal runs 150)
         x.whole_from = r <= 32 ? ~0u : std::max(1u, dev.compute_units * 3 / 4);
     };
     char* ws = static_cast<char*>(dev.workspace);
@@ -385,7 +394,8 @@ int Planner::verify() {
     a.u_accept = P<float>(n + 2); a.u_sample = P<float>(n + 3); a.temperature = P<float>(n + 4);
     a.tokens = P<int32_t>(n + 5); a.counts = P<int32_t>(n + 6);
     a.vector = a.stride % 8 == 0 && aligned16(a.target) && (given || aligned16(a.draft)) ? 1u : 0u;
-    // runs of 512 logits up to 4096, as long as there are eight waves a compute unit
+    // runs of 512 logits up to 4096, as long as there are eight waves a compute unit (five rows of 151936: 26 us with runs of 512, 29
+    // with runs of 4096)
     a.span = kVerifyMaxSpan;
     while (a.span > kVerifyStep && (uint64_t)a.rows * n * ((a.vocab + a.span - 1) / a.span) < 8ull * dev.compute_units) a.span /= 2;
     a.runs = (a.vocab + a.span - 1) / a.span;
