@@ -297,3 +297,34 @@ def test_infinities_in_keys_before_every_rows_window(ctx, dtype, dim, n):
 @pytest.mark.parametrize("tokens,heads,kv_heads,prefix", [(600, 32, 4, 1700), (300, 64, 64, 200)])
 def test_a_prefix_behind_many_sequences(ctx, tokens, heads, kv_heads, prefix):
     Case(ctx, fx.BF16, [1] * tokens, [1 + s % 5 for s in range(tokens)], heads, kv_heads, 64, 64, prefix=prefix, pad=3).run()
+
+
+@pytest.mark.parametrize("n", [1, 70])
+def test_caches_past_four_gigabytes(n):
+    """Pages beyond 2^32 bytes and 2^31 values into keys and values, put away and read."""
+    dim, kv, heads, page, pages, own = 256, 8, 16, 256, 4200, 300
+    places = np.array([4199, 3, 4198], np.int32)
+    rng = fx.rng_for(230, n)
+    kb, k = sr.values(rng, (own, kv, dim), fx.BF16)
+    vb, v = sr.values(rng, (own, kv, dim), fx.BF16)
+    qb, q = sr.values(rng, (n, heads, dim), fx.BF16, 2.0)
+    j = np.arange(own)
+    ctx = rt.Context()
+    try:
+        ctx.put(1, kb); ctx.put(2, vb); ctx.put(3, j.astype(np.int32)); ctx.put(4, (places[j // page] * page + j % page).astype(np.int32)); ctx.put(5, np.zeros(1))
+        ctx.alloc(6, pages * page * kv * dim * 2); ctx.alloc(7, pages * page * kv * dim * 2)
+        ctx.put(8, qb); ctx.put(9, places); ctx.put(10, np.array([own], np.int32)); ctx.put(11, np.array([0, n], np.int32)); ctx.alloc(12, n * heads * dim * 2)
+        em = cc.Emitter(act_dtype=ACT[fx.BF16])
+        em.paged_kv_append(B(1), B(2), B(3), B(4), B(5), B(6), B(7), own, kv, dim, 0, page, pages)
+        em.paged_attention(B(8), B(6), B(7), B(9), B(10), B(11), B(12), n, 1, heads, kv, dim, page, pages, len(places), dim ** -0.5)
+        ctx.interpret_decode(em.table_for(ctx))
+        ctx.wait()
+        got = sr.wide(ctx.read(12, np.uint16, n * heads * dim), fx.BF16).reshape(n, heads, dim)
+    finally:
+        ctx.close()
+    # the same sequence in a pool of two pages
+    small = [np.zeros((2, kv, page, dim)) for _ in range(2)]
+    for x, rows in zip(small, (k, v)):
+        x[j // page, :, j % page] = rows
+    y, reach, sharp, count = sr.attention(q, *small, 2, np.array([[0, 1]]), [own], [0, n], float(np.float32(dim ** -0.5)), 0, np.zeros(0, np.int32), 0)
+    assert np.all(np.abs(got - y) <= sr.attention_tolerance(y, reach, sharp, count, dim, fx.BF16))
