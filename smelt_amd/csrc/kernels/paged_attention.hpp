@@ -431,8 +431,8 @@ __device__ __forceinline__ void attn_clear(AttnAcc<D>& acc) {
 
 // Values are multiplied with a zero probability where one of a tile's rows does not see a key and another does, and a zero does not silence
 // an infinity or a NaN.  Rows that came out as NaN are therefore formed once more at a segment's end, key after key (maxima and sums
-// are right: hidden scores are taken out before those).  Slow, and outside of the key loops, which looking for such values cost a fifth
-// of their time.
+// are right: hidden scores are taken out before those).  That is slow and rare, and stands outside of the key loops: a search for such
+// values within them cost a fifth of their time.
 //
 // Calls use(whether a row of the given bounds sees it, the first 8 dims of its K, its V row) for the keys of the workgroup's part of a
 // segment.
