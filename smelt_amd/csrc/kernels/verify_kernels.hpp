@@ -334,7 +334,10 @@ __device__ __forceinline__ VerifyInverse verify_inverse(const VerifyArgs& a, uin
     return VerifyInverse{ps > 0.0 ? 1.0 / ps : 0.0, ds > 0.0 ? 1.0 / ds : 0.0};
 }
 
+// The leftover weight max(p - q, 0) of a token.  Both products are rounded before the difference, so that equal rows leave exactly nothing
+// over (a fused multiply-add would leave the rounding of one of them, and a token would be drawn from that).
 __device__ __forceinline__ double verify_rest(const VerifyExp& e, float x, float y, const VerifyChoice& c, const VerifyInverse& inv, double rate) {
+#pragma clang fp contract(off)
     return __builtin_fmax(e.weight(x, c.top, rate) * inv.p - e.weight(y, c.draft_top, rate) * inv.d, 0.0);
 }
 
@@ -459,8 +462,8 @@ __device__ __forceinline__ void verify_draw(const VerifyArgs& a) {
             for (uint32_t k = 0; k < E; ++k) {
                 w[k] = 0.0;
                 if (k < each) {
-                    const double p = e.weight(verify_logit(x[k]), c.top, q.rate64);
-                    const double v = two && rest ? __builtin_fmax(p * inv.p - e.weight(verify_logit(y[k]), c.draft_top, q.rate64) * inv.d, 0.0) : p;
+                    const float logit = verify_logit(x[k]);
+                    const double v = two && rest ? verify_rest(e, logit, verify_logit(y[k]), c, inv, q.rate64) : e.weight(logit, c.top, q.rate64);
                     w[k] = i0 + k < end && (int32_t)(i0 + k) != without ? v : 0.0;
                 }
                 sum += w[k];

@@ -196,3 +196,24 @@ def test_verify_is_refused_where_a_slot_is_short(ctx):
         with pytest.raises(rt.SmeltHipError, match="needs"):
             go(**kw)
     ctx.wait()
+
+
+@TYPES
+@pytest.mark.parametrize("vocab", [500, 32000])
+@pytest.mark.parametrize("flat", [False, True], ids=["normal", "flat"])
+def test_a_draft_model_that_is_the_target_leaves_nothing_over(ctx, dtype, vocab, flat):
+    """p == q, and a draft that is refused all the same (outside the vocabulary, masked in both rows, u_accept of 1): max(p - q, 0) is zero
+    everywhere, so the token is drawn from p."""
+    us = [0.0, 0.03, 0.2, 0.37, 0.5, 0.61, 0.8, 0.97, 1.0 - 2.0 ** -24]
+    c = batch(fx.rng_for(243, vocab), dtype, [2] * len(us), vocab)
+    if flat:
+        c["target"][:] = fx.to_bits(np.float32([1.5]), dtype)[0]
+    c["target"][:, 17] = 0xFC00 if dtype == fx.F16 else 0xFF80
+    c["draft"] = c["target"].copy()
+    c["us"][:] = us
+    first = c["offsets"][:-1]
+    for drafted, u in ((-1, 0.0), (vocab, 0.5), (17, 0.0), (40, 1.0)):
+        c["drafts"][first] = drafted
+        c["ua"][first] = u
+        _, counts = check(ctx, c)
+        assert not counts.any()
