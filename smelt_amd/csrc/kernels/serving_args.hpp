@@ -137,7 +137,9 @@ SMELT_HD AttentionSpan attention_span(const AttentionArgs& a, const AttentionEnt
     const uint32_t last = (first + count - 1) / a.group;
     const int32_t p0 = zero + (int32_t)(first / a.group), p1 = zero + (int32_t)(last < e.tokens ? last : e.tokens - 1);
     AttentionSpan s{0, p1 + 1, 0, p0 + 1};
-    if (a.window) { s.lo = p0 - (int32_t)a.window + 1; s.all_lo = p1 - (int32_t)a.window + 1; }
+    // (a window that a position is within hides nothing of it; the differences stay at 0 and above)
+    if (a.window && p0 >= (int32_t)a.window) s.lo = p0 - (int32_t)a.window + 1;
+    if (a.window && p1 >= (int32_t)a.window) s.all_lo = p1 - (int32_t)a.window + 1;
     return s;
 }
 

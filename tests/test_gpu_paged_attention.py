@@ -328,3 +328,14 @@ def test_caches_past_four_gigabytes(n):
         x[j // page, :, j % page] = rows
     y, reach, sharp, count = sr.attention(q, *small, 2, np.array([[0, 1]]), [own], [0, n], float(np.float32(dim ** -0.5)), 0, np.zeros(0, np.int32), 0)
     assert np.all(np.abs(got - y) <= sr.attention_tolerance(y, reach, sharp, count, dim, fx.BF16))
+
+
+# (the reference's differences of 32-bit numbers overflow for rows before key 0, which see nothing either way)
+@pytest.mark.filterwarnings("ignore:overflow encountered")
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,own,prefix", [(80, 70, 0), (200, 190, 0), (60, 20, 0), (90, 70, 3), (20, 15, 0)])
+def test_a_window_of_everything_hides_nothing(ctx, dtype, dim, n, own, prefix):
+    """The widest window there is, with fewer keys than rows: the result of no window, bit for bit."""
+    got = [Case(ctx, dtype, [n, 1], [own, 30], 2, 2, dim, 16, prefix=prefix, window=window).run().result() for window in (2 ** 31 - 1, 0)]
+    assert np.array_equal(*got)

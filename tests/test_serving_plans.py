@@ -293,3 +293,14 @@ def test_launches_that_are_too_wide_are_refused():
                pages_per_sequence=1, scale=0.1)
     em.paged_attention(**att, tokens=10_000_000, sequences=100)
     refused(lambda: em.paged_attention(**att, tokens=33_000_000, sequences=200_000), "threads")
+
+
+@pytest.mark.parametrize("part", [WHOLE, OWN])
+@pytest.mark.parametrize("prefix", [0, 20])
+def test_the_widest_windows_hide_nothing(partition, part, prefix):
+    """Windows up to 2^31 - 1, also where rows stand before the first key (fewer keys than rows): the key tiles of no window."""
+    for n, own, group, row_tile in ((80, 70, 1, 128), (80, 70, 6, 256), (300, 2, 1, 32), (40, 0, 2, 16), (1, 1, 1, 32), (9, 500, 4, 32)):
+        a = dict(offsets=[0, n], lens=[own], tokens=n, group=group, width=64, prefix=prefix, prefix_pages=7, part=part, row_tile=row_tile)
+        want = entries(partition, **a)[0]
+        for window in (1000, 2 ** 30, 2 ** 31 - n, 2 ** 31 - 2, 2 ** 31 - 1):
+            assert entries(partition, **a, window=window)[0] == want, (n, own, group, row_tile, window)
