@@ -292,17 +292,14 @@ __device__ __forceinline__ void verify_choose(const VerifyArgs& a) {
     const uint32_t first = run * a.span, last = first + a.span < a.vocab ? first + a.span : a.vocab;
     const int32_t without = !a.draft && leftover ? a.draft_tokens[row] : -1;
     double* out = a.sums + (size_t)s * 3 * a.runs + run;
-    double sum = 0.0, dsum = 0.0, dropped = 0.0;
+    double sum = 0.0, dsum = 0.0;
     const uint16_t* target = a.target + (size_t)row * a.stride;
     const uint16_t* draft = two ? a.draft + (size_t)row * a.stride : nullptr;
     const VerifyExp e;
+    // (a refused draft that was given is left out of the sum: taking it away afterwards would take the small weights beside it along)
     auto add = [&](uint32_t i, const float* x) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const double w = e.weight(x[k], top, q.rate64);
-            sum += w;
-            dropped = (int32_t)(i + k) == without ? w : dropped;
-        }
+        for (int k = 0; k < 8; ++k) sum += e.weight((int32_t)(i + k) == without ? -__builtin_inff() : x[k], top, q.rate64);
     };
     if (two)
         verify_walk<ActT, true>(target, draft, first, last, a.vector, [&](uint32_t i, const float* x, const float* y) {
@@ -315,11 +312,11 @@ __device__ __forceinline__ void verify_choose(const VerifyArgs& a) {
     // (a row without any weight: its top is -inf and the differences above are not numbers, which weigh nothing)
     sum = wave_total(sum);
     if (two) dsum = wave_total(dsum);
-    dropped = wave_total(dropped);
     if (lane == 0) {
-        out[0] = sum;
+        const bool here = without >= 0 && (uint32_t)without >= first && (uint32_t)without < last;
+        out[0] = here ? sum + e.weight(verify_logit(ActT::widen(target[(uint32_t)without])), top, q.rate64) : sum;
         if (two) out[a.runs] = dsum;
-        out[2 * a.runs] = without >= 0 && (uint32_t)without >= first && (uint32_t)without < last ? __builtin_fmax(sum - dropped, 0.0) : sum;
+        out[2 * a.runs] = sum;
     }
 }
 

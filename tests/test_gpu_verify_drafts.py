@@ -217,3 +217,25 @@ def test_a_draft_model_that_is_the_target_leaves_nothing_over(ctx, dtype, vocab,
         c["ua"][first] = u
         _, counts = check(ctx, c)
         assert not counts.any()
+
+
+@TYPES
+@pytest.mark.parametrize("vocab", [9, 400, 3000, 32000])
+def test_what_a_certain_draft_leaves_over(ctx, dtype, vocab):
+    """A looked-up draft that holds all but 2^-60 of the probability and is refused (u_accept of 1): the token is drawn from the others, however
+    little they hold; from p where they hold nothing."""
+    us = [0.0, 0.1, 0.25, 0.5, 0.77, 1.0 - 2.0 ** -24]
+    c = batch(fx.rng_for(244, vocab), dtype, [2] * len(us), vocab, given=True)
+    first = c["offsets"][:-1]
+    for at in (0, 5, vocab - 1):
+        for others in (1.0, 0.0):
+            t = sr.wide(c["target"], dtype) - 60.0
+            if not others:
+                t[first] = -np.inf
+            t[first, at] = 0.0
+            c["target"] = fx.to_bits(t.astype(np.float32), dtype)
+            c["temperature"][:], c["us"][:] = 1.0, us
+            c["drafts"][first], c["ua"][first] = at, 1.0
+            tokens, counts = check(ctx, c)
+            assert not counts.any() and np.all((tokens[first] == at) == (others == 0.0))
+            c = batch(fx.rng_for(244, vocab), dtype, [2] * len(us), vocab, given=True)
