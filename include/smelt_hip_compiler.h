@@ -239,7 +239,8 @@ typedef struct SmeltRopeScaling {
 int smelt_rope_table(const SmeltRopeScaling *scaling, int rotary_dim, double *out_table, float *out_amplitude);
 
 /* "rope_{half,interleaved}_d{D}_r{R}": `tokens` rows of `heads` heads, strides in elements (>= heads * head_dim).  Output may be the
- * input itself (same slot, offset and stride); other overlaps are refused. */
+ * input itself (same slot, offset and stride), or lie beside it within the same rows; other overlaps are refused.  (Rows at equal strides
+ * overlap where they share a byte, rows at different ones where what they span does.) */
 int smelt_emit_rope(smelt_emitter *e, const SmeltRope *rope, SmeltBinding input, SmeltBinding output,
                     SmeltBinding positions, SmeltBinding table, int heads, int input_stride,
                     int output_stride, int tokens, int dynamic);
@@ -255,7 +256,8 @@ typedef struct SmeltPagedCache {
 /* "paged_kv_append[_q]_{half,interleaved}_d{D}_r{R}_kv{H}_p{P}": token rows k (rotated) and v put to place slots[token] = page *
  * page_size + offset; a negative slot, or one behind the pool, puts the token nowhere.  Tokens that name the same place leave one of
  * them, element by element unspecified which.  With q and q_out (both or neither) the q rows are rotated in the same launch,
- * also those of tokens without a place; q_out may be q itself.  rotary_dim 0 rotates nothing. */
+ * also those of tokens without a place; q_out may be q itself, also within rows [q | k | v] that one projection wrote.  rotary_dim 0
+ * rotates nothing. */
 int smelt_emit_paged_kv_append(smelt_emitter *e, const SmeltRope *rope, const SmeltPagedCache *cache,
                                SmeltBinding k, SmeltBinding v, SmeltBinding positions,
                                SmeltBinding slots, SmeltBinding table, const SmeltBinding *q,

@@ -119,7 +119,15 @@ struct Planner {
     float F(size_t i) const { float f; memcpy(&f, &value[i], 4); return f; }
     template <class T> T* P(int i) const { return static_cast<T*>(plan->operand[i].ptr); }
     void need(int i, size_t bytes, size_t align = 2, bool written = false) {
-        plan->operand[i].need = bytes; plan->operand[i].align = align; plan->operand[i].written = written;
+        ServingOperand& o = plan->operand[i];
+        o.need = bytes; o.align = align; o.written = written;
+        o.row = o.stride = 0;
+    }
+    // `tokens` rows of `count` 16-bit values at `stride`
+    void need_rows(int i, uint32_t tokens, uint32_t count, uint32_t stride, bool written = false) {
+        need(i, row_bytes(tokens, count, stride), 2, written);
+        plan->operand[i].row = (size_t)count * 2;
+        plan->operand[i].stride = (size_t)stride * 2;
     }
     template <class A> ServingStep& step(int kernel, const A& args, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t threads, size_t lds) {
         static_assert(sizeof(A) <= kServingArgBytes, "argument block");
@@ -135,15 +143,27 @@ struct Planner {
     }
     // bytes of `tokens` rows of `count` 16-bit values at `stride`
     static size_t row_bytes(uint32_t tokens, uint32_t count, uint32_t stride) { return tokens ? ((size_t)(tokens - 1) * stride + count) * 2 : 0; }
+    // Whether two operands share a byte.  Rows at one stride (q, k and v within the rows of a fused projection) are compared row by row: row
+    // j of y lies distance + (j - i) * stride behind row i of x, and the least j - i is looked for that is not wholly before it.
+    static bool meet(const ServingOperand& x, const ServingOperand& y) {
+        const char *a = static_cast<const char*>(x.ptr), *b = static_cast<const char*>(y.ptr);
+        if (!(a < b + y.need && b < a + x.need)) return false;
+        if (x.stride == 0 || x.stride != y.stride) return true;
+        typedef __int128 wide;
+        const wide stride = x.stride, distance = (wide)(intptr_t)b - (wide)(intptr_t)a, from = -(wide)y.row - distance;
+        const wide rows_x = (x.need - x.row) / x.stride, rows_y = (y.need - y.row) / y.stride;      // less one each
+        wide k = (from >= 0 ? from / stride : -((-from + stride - 1) / stride)) + 1;
+        k = k > -rows_x ? k : -rows_x;
+        return k <= rows_y && distance + k * stride < (wide)x.row;
+    }
     // operand `w` is written: it must not overlap any other one, but for `same`, which may be the very same rows
     int apart(int w, int same = -1, bool same_rows = false) {
-        const char* lo = P<char>(w);
-        const char* hi = lo + plan->operand[w].need;
+        const ServingOperand& o = plan->operand[w];
         for (int i = 0; i < plan->operands; ++i) {
-            const char* p = P<char>(i);
-            if (i == w || plan->operand[i].need == 0 || lo == hi) continue;
-            if (i == same && same_rows && p == lo) continue;
-            if (p < hi && lo < p + plan->operand[i].need)
+            const ServingOperand& x = plan->operand[i];
+            if (i == w || x.need == 0 || o.need == 0) continue;
+            if (i == same && same_rows && x.ptr == o.ptr) continue;
+            if (meet(o, x))
                 return fail(SMELT_HIP_ERR_INVALID_ARGUMENT, "output argument " + std::to_string(w) + " overlaps argument " + std::to_string(i));
         }
         return 0;
@@ -174,8 +194,8 @@ int Planner::rope() {
         a.q.src = P<uint16_t>(0); a.q.dst = P<uint16_t>(1);
         a.q.src_stride = U(o + 2); a.q.dst_stride = U(o + 3);
         a.table = P<double>(3);
-        need(0, row_bytes(a.tokens, q_heads * a.dim, a.q.src_stride));
-        need(1, row_bytes(a.tokens, q_heads * a.dim, a.q.dst_stride), 2, true);
+        need_rows(0, a.tokens, q_heads * a.dim, a.q.src_stride);
+        need_rows(1, a.tokens, q_heads * a.dim, a.q.dst_stride, true);
         need(2, (size_t)a.tokens * 4, 4);
         need(3, (size_t)half * 8, 8);
     } else {
@@ -191,8 +211,8 @@ int Planner::rope() {
         a.k.heads = a.v.heads = kv_heads;
         if (a.pages == 0 || (uint64_t)a.pages * page > 0x7FFFFFFFull) return bad("the pool must hold 1 to 2^31 - 1 tokens");
         const size_t cache = (size_t)a.pages * page * kv_heads * a.dim * 2;
-        need(0, row_bytes(a.tokens, kv_heads * a.dim, a.k.src_stride));
-        need(1, row_bytes(a.tokens, kv_heads * a.dim, a.v.src_stride));
+        need_rows(0, a.tokens, kv_heads * a.dim, a.k.src_stride);
+        need_rows(1, a.tokens, kv_heads * a.dim, a.v.src_stride);
         need(2, half ? (size_t)a.tokens * 4 : 0, 4);
         need(3, (size_t)a.tokens * 4, 4);
         need(4, (size_t)half * 8, 8);
@@ -202,8 +222,8 @@ int Planner::rope() {
             q_heads = U(o + 5);
             a.q.src = P<uint16_t>(7); a.q.dst = P<uint16_t>(8);
             a.q.src_stride = U(o + 6); a.q.dst_stride = U(o + 7);
-            need(7, row_bytes(a.tokens, q_heads * a.dim, a.q.src_stride));
-            need(8, row_bytes(a.tokens, q_heads * a.dim, a.q.dst_stride), 2, true);
+            need_rows(7, a.tokens, q_heads * a.dim, a.q.src_stride);
+            need_rows(8, a.tokens, q_heads * a.dim, a.q.dst_stride, true);
         }
         if (a.k.src_stride < kv_heads * a.dim || a.v.src_stride < kv_heads * a.dim) return bad("a row stride is shorter than its heads");
     }
@@ -270,7 +290,7 @@ int Planner::attention() {
     a.scale_log2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 1.2e-38f);
     a.flip_q = scale < 0.0f ? 0x80008000u : 0u;
     const size_t cache = (size_t)a.pages * page * a.kv_heads * dim * 2;
-    need(0, row_bytes(a.tokens, a.heads * dim, a.q_stride));
+    need_rows(0, a.tokens, a.heads * dim, a.q_stride);
     need(1, cache, 16);
     need(2, cache, 16);
     need(3, (size_t)a.sequences * a.pages_per_sequence * 4, 4);
@@ -377,8 +397,8 @@ int Planner::verify() {
     if (a.vocab == 0 || a.vocab > 0x7FFFFFF0u) return bad("the vocabulary must hold 1 to 2^31 - 17 tokens");
     if (a.stride < a.vocab) return bad("the row stride is shorter than the vocabulary");
     if (a.rows > 65535 || a.sequences > 65535) return bad("at most 65535 rows and sequences");
-    need(0, row_bytes(a.rows, a.vocab, a.stride));
-    if (!given) need(1, row_bytes(a.rows, a.vocab, a.stride));
+    need_rows(0, a.rows, a.vocab, a.stride);
+    if (!given) need_rows(1, a.rows, a.vocab, a.stride);
     need(n, (size_t)a.rows * 4, 4);
     need(n + 1, ((size_t)a.sequences + 1) * 4, 4);
     need(n + 2, (size_t)a.rows * 4, 4);

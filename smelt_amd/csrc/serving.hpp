@@ -17,6 +17,7 @@ struct ServingOperand {
     size_t need = 0;            // bytes the launch touches from ptr on
     size_t align = 2;
     bool written = false;
+    size_t row = 0, stride = 0; // rows: bytes of one and from one to the next (0: the bytes lie in one run)
 };
 
 constexpr int kServingMaxOperands = 16;

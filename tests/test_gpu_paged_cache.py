@@ -140,3 +140,33 @@ def test_slots_bound_to_the_callers_memory(ctx):
     finally:
         ctx.wait()
         hip.hipFree(p)
+
+
+@pytest.mark.parametrize("dtype", [fx.F16, fx.BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
+@pytest.mark.parametrize("tokens,kv,h,dim,rot,gap", [(1, 2, 8, 64, 64, 0), (2, 4, 24, 256, 64, 0), (64, 2, 8, 128, 128, 16), (29, 1, 5, 64, 20, 3), (1100, 2, 4, 64, 64, 0)])
+def test_append_with_q_in_place_within_fused_rows(ctx, dtype, interleaved, tokens, kv, h, dim, rot, gap):
+    """Rows [q | k | v] of one buffer: q rotated where it stands, k and v read beside it and left as they were."""
+    rng = fx.rng_for(212, tokens + dim + rot)
+    page, q_end, k_end, row = 16, h * dim, (h + kv) * dim, (h + 2 * kv) * dim + gap
+    pages = -(-tokens // page) + 1
+    bits, x = sr.values(rng, (tokens, row), dtype)
+    slots, positions = rng.permutation(pages * page)[:tokens].astype(np.int32), rng.integers(0, 200000, tokens).astype(np.int32)
+    table, _ = cc.rope_table(rot)
+    for slot, a in ((1, bits), (3, positions), (4, slots), (5, table)):
+        ctx.put(slot, a)
+    ctx.alloc(6, pages * page * kv * dim * 2); ctx.alloc(7, pages * page * kv * dim * 2)
+    em = cc.Emitter(act_dtype=ACT[dtype])
+    em.paged_kv_append(B(1, 2 * q_end), B(1, 2 * k_end), B(3), B(4), B(5), B(6), B(7), tokens, kv, dim, rot, page, pages, interleaved=interleaved, kv_stride=row, q=B(1), q_out=B(1), q_heads=h,
+                       q_stride=row, q_out_stride=row)
+    assert ctx.interpret_decode(em.table_for(ctx)) == 1
+    ctx.wait()
+    got = ctx.read(1, np.uint16, bits.size).reshape(bits.shape)
+    assert np.array_equal(got[:, q_end:], bits[:, q_end:])
+    want, reach = sr.rope(x[:, :q_end].reshape(tokens, h, dim), positions, table, 1.0, rot, interleaved)
+    sr.check_rope(got[:, :q_end], want, reach, dtype, "q")
+    at, off = slots // page, slots % page
+    assert np.array_equal(ctx.read(7, np.uint16, pages * page * kv * dim).reshape(pages, kv, page, dim)[at, :, off], bits[:, k_end:k_end + kv * dim].reshape(tokens, kv, dim))
+    want, reach = sr.rope(x[:, q_end:k_end].reshape(tokens, kv, dim), positions, table, 1.0, rot, interleaved)
+    placed = sr.keys_from_pages(ctx.read(6, np.uint16, pages * page * kv * dim).reshape(pages, kv, dim // 8, page, 8))[at, :, off]
+    sr.check_rope(placed, want, reach, dtype, "keys")

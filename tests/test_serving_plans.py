@@ -304,3 +304,56 @@ def test_the_widest_windows_hide_nothing(partition, part, prefix):
         want = entries(partition, **a)[0]
         for window in (1000, 2 ** 30, 2 ** 31 - n, 2 ** 31 - 2, 2 ** 31 - 1):
             assert entries(partition, **a, window=window)[0] == want, (n, own, group, row_tile, window)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 64])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_q_is_rotated_in_place_within_fused_rows(tokens, interleaved):
+    """Rows [q | k | v] of one projection: q_out may be q itself, or rows elsewhere in the fused ones that no other operand has."""
+    em, (h, kv, d) = cc.Emitter(), (8, 2, 64)
+    row = (h + 2 * kv) * d
+
+    def go(q_at=0, q_out_at=0, k_at=h * d, v_at=(h + kv) * d, stride=row, q_out_stride=None, q_out_slot=1, **kw):
+        em.paged_kv_append(B(1, 2 * k_at), B(1, 2 * v_at), B(3), B(4), B(5), B(6), B(7), tokens=tokens, kv_heads=kv, head_dim=d, rotary_dim=d, page_size=16, pages=10, kv_stride=stride,
+                           q=B(1, 2 * q_at), q_out=B(q_out_slot, 2 * q_out_at), q_heads=h, q_stride=stride, q_out_stride=stride if q_out_stride is None else q_out_stride,
+                           interleaved=interleaved, **kw)
+
+    go()
+    go(q_at=2 * kv * d, q_out_at=2 * kv * d, k_at=0, v_at=kv * d)                  # [k | v | q]
+    go(q_at=kv * d, q_out_at=kv * d, k_at=0, v_at=(h + kv) * d)                    # [k | q | v]
+    go(stride=row + 8)
+    go(stride=2 * row, q_out_at=row)                                              # columns of their own
+    refused(lambda: go(k_at=h * d - 1), "overlaps")                               # one value of q is k's
+    refused(lambda: go(q_out_at=kv * d), "overlaps")                              # q's rows, but not the same ones
+    refused(lambda: go(stride=2 * row, q_out_at=row - 1), "overlaps")
+    if tokens > 1:
+        refused(lambda: go(q_out_stride=row + 8), "overlaps")
+        refused(lambda: go(q_out_at=row), "overlaps")                             # a row down: where later rows of q are
+    refused(lambda: go(q_out_slot=6), "overlaps")
+    em.rope(B(1), B(1), B(3), B(4), tokens, h, d, d, x_stride=row, y_stride=row)
+    em.rope(B(1, 2 * h * d), B(1, 2 * h * d), B(3), B(4), tokens, kv, d, d, x_stride=row, y_stride=row)
+    em.rope(B(1, 2 * h * d), B(1, 2 * (h + kv) * d), B(3), B(4), tokens, kv, d, d, x_stride=row, y_stride=row)
+
+
+def test_rows_overlap_where_they_share_a_byte():
+    """What is refused, against the sets of values that the rows hold."""
+    em = cc.Emitter()
+    dim, seen = 2, set()
+    for tokens in (1, 2, 3):
+        for heads in (1, 2):
+            for stride in range(heads * dim, 8):
+                for stride_y in (stride, stride + 1):
+                    for x in (0, 13):
+                        for y in range(0, 30):
+                            rows = [{at + t * s + i for t in range(tokens) for i in range(heads * dim)} for at, s in ((x, stride), (y, stride_y))]
+                            overlap = bool(rows[0] & rows[1]) and not (x == y and stride == stride_y)
+                            span = [range(min(r), max(r) + 1) for r in rows]
+                            if stride != stride_y and span[0][0] <= span[1][-1] and span[1][0] <= span[0][-1]:
+                                overlap = True                                     # (different strides: the runs are compared)
+                            call = lambda: em.rope(B(1, 2 * x), B(1, 2 * y), B(3), B(4), tokens, heads, dim, dim, x_stride=stride, y_stride=stride_y)   # noqa: E731
+                            if overlap:
+                                refused(call, "overlaps")
+                            else:
+                                call()
+                            seen.add(overlap)
+    assert seen == {False, True}
