@@ -257,8 +257,11 @@ def plan_matvec(layout, rows, cols, group, nmat=1, lds_limit=160 * 1024, force=F
     return dict(zip(MATVEC_PLAN_FIELDS, out)) if rc else None
 
 
-def rope_table(rotary_dim, base=10000.0, kind=ROPE_PLAIN, factor=1.0, positions=8192.0, low=1.0, high=4.0):
-    """(radians a position of each pair as float64, amplitude) for a rotation scaled to longer contexts."""
+def rope_table(rotary_dim, base=10000.0, kind=ROPE_PLAIN, factor=1.0, positions=8192.0, low=1.0, high=None):
+    """(radians a position of each pair as float64, amplitude) for a rotation scaled to longer contexts.  `high` turns are kept as they
+    are: 4 of bands, 32 of parts when it is not given."""
+    if high is None:
+        high = 32.0 if kind == ROPE_PARTS else 4.0
     out = np.zeros(max(rotary_dim // 2, 1), np.float64)
     amplitude = C.c_float(1.0)
     rc = lib().smelt_rope_table(C.byref(RopeScaling(kind, base, factor, positions, low, high)), rotary_dim,

@@ -357,3 +357,11 @@ def test_rows_overlap_where_they_share_a_byte():
                                 call()
                             seen.add(overlap)
     assert seen == {False, True}
+
+
+def test_rope_table_defaults():
+    """What each scaling keeps when the caller does not say: 1 to 4 turns of bands, 1 to 32 of parts."""
+    same = lambda kind, high: np.array_equal(cc.rope_table(128, kind=kind, factor=4.0)[0], cc.rope_table(128, kind=kind, factor=4.0, positions=8192.0, low=1.0, high=high)[0])   # noqa: E731
+    assert same(cc.ROPE_BANDS, 4.0) and not same(cc.ROPE_BANDS, 32.0)
+    assert same(cc.ROPE_PARTS, 32.0) and not same(cc.ROPE_PARTS, 4.0)
+    assert not np.array_equal(cc.rope_table(128, kind=cc.ROPE_PARTS, factor=4.0, high=8.0)[0], cc.rope_table(128, kind=cc.ROPE_PARTS, factor=4.0)[0])
