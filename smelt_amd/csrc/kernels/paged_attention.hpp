@@ -432,7 +432,9 @@ __device__ __forceinline__ void attn_clear(AttnAcc<D>& acc) {
 // Values are multiplied with a zero probability where one of a tile's rows does not see a key and another does, and a zero does not silence
 // an infinity or a NaN.  Rows that came out as NaN are therefore formed once more at a segment's end, key after key (maxima and sums
 // are right: hidden scores are taken out before those).  That is slow and rare, and stands outside of the key loops: a search for such
-// values within them cost a fifth of their time.
+// values within them cost a fifth of their time.  A row whose sum is a NaN has seen a score that is one (a NaN in q or in a key, or an infinite
+// score): its answer is NaN and it is left as it is (one sequence of NaN among 64 that decode 83 us, as without it, and 15 ms when its rows
+// were formed again; one of two prompt chunks 159 us and 82 ms).
 //
 // Calls use(whether a row of the given bounds sees it, the first 8 dims of its K, its V row) for the keys of the workgroup's part of a
 // segment.
@@ -676,7 +678,7 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
                 sum += f * sh.l[w][r];
             }
             const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
-            if (__builtin_expect(y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w, 0)) {
+            if (__builtin_expect(sum == sum && (y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w), 0)) {
                 const uint16_t* q = a.q + (size_t)token * a.q_stride + (size_t)head * D;
                 const float shift = top == -__builtin_inff() ? 0.0f : -top * scale.c;
                 y = float4_t{0, 0, 0, 0};
@@ -947,7 +949,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) nan = nan || acc.o[j][i] != acc.o[j][i];
-        const unsigned long long nans = __ballot(nan && row.live);
+        const unsigned long long nans = __ballot(nan && l == l && row.live);
         const uint32_t again = (uint32_t)nans | (uint32_t)(nans >> 32);          // rows
         const bool done = !((again >> (lane & 31)) & 1u);
         if (row.live) {

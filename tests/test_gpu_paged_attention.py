@@ -339,3 +339,37 @@ def test_a_window_of_everything_hides_nothing(ctx, dtype, dim, n, own, prefix):
     """The widest window there is, with fewer keys than rows: the result of no window, bit for bit."""
     got = [Case(ctx, dtype, [n, 1], [own, 30], 2, 2, dim, 16, prefix=prefix, window=window).run().result() for window in (2 ** 31 - 1, 0)]
     assert np.array_equal(*got)
+
+
+def timed(case, table, repeats=5):
+    best = np.inf
+    for _ in range(repeats):
+        case.ctx.interpret_decode(table)
+        case.ctx.wait()
+        best = min(best, case.ctx.last_gpu_ns() / 1000.0)
+    return best
+
+
+# decoding and a prompt behind a few thousand keys: a row of NaN in q, or in a key that all rows see
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,own,prefix", [([1, 1, 2], [3000, 40, 700], 0), ([1, 1, 2], [3000, 40, 700], 500), ([300, 70], [2500, 90], 0), ([300, 70], [2500, 90], 500)])
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_rows_whose_scores_are_nan(ctx, dtype, dim, n, own, prefix, where):
+    """They are NaN, the other rows are as they were bit for bit, and the batch takes as long as it did (a row formed a second time takes
+    hundreds of times as long)."""
+    c = Case(ctx, dtype, n, own, 8, 2, dim, 64, prefix=prefix, poison=False)
+    table = c.load()
+    clean = timed(c, table)
+    before = c.result().copy()
+    nan = 0x7E00 if dtype == fx.F16 else 0x7FC0
+    if where == "q":
+        c.qb[:n[0]] = nan
+    else:
+        c.kb[c.table[0, 0], :, 2] = nan
+    table = c.load()
+    took = timed(c, table)
+    got, rows = c.result(), slice(0, n[0])
+    assert np.isnan(sr.wide(got[rows], dtype)).all()
+    assert np.array_equal(got[n[0]:], before[n[0]:])
+    assert took < 3 * clean + 50, f"{took:.0f} us, {clean:.0f} before"
