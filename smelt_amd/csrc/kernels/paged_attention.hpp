@@ -430,31 +430,132 @@ __device__ __forceinline__ void attn_clear(AttnAcc<D>& acc) {
 }
 
 // Values are multiplied with a zero probability where one of a tile's rows does not see a key and another does, and a zero does not silence
-// an infinity or a NaN.  Rows that came out as NaN are therefore formed once more at a segment's end, key after key (maxima and sums
-// are right: hidden scores are taken out before those).  That is slow and rare, and stands outside of the key loops: a search for such
-// values within them cost a fifth of their time.  A row whose sum is a NaN has seen a score that is one (a NaN in q or in a key, or an infinite
-// score): its answer is NaN and it is left as it is (one sequence of NaN among 64 that decode 83 us, as without it, and 15 ms when its rows
-// were formed again; one of two prompt chunks 159 us and 82 ms).
-//
-// Calls use(whether a row of the given bounds sees it, the first 8 dims of its K, its V row) for the keys of the workgroup's part of a
-// segment.
-template <int D, class Bounds, class Use>
-__device__ __forceinline__ void attn_each_key(const AttentionArgs& a, const AttentionEntry& e, const AttnSegment& g, Bounds bounds, Use use) {
+// an infinity or a NaN.  Rows that came out as NaN are therefore formed once more at a segment's end, over the keys they see (maxima and
+// sums are right: hidden scores are taken out before those).  That is rare and stands outside of the key loops: a search for such values
+// within them cost a fifth of their time.  Two kinds of rows are left as they are, since NaN is their answer.  A row whose sum is a NaN has
+// seen a score that is one (a NaN in q or in a key, or an infinite score).  And where every value that is not finite is a NaN that all of the
+// tile's rows see, it is theirs.  One sequence with a NaN among many: 64 that decode 83 us for a score and 87 for a value, as without
+// either; four with 50000 to 65536 keys 182 and 220 (without 182); two prompt chunks 150 and 380 (150), and 14600 for a value in the
+// last key, whose tile's other 255 rows are formed again; drafted tokens 66 and 66 (66), 330 for one in the last key.
+
+// The keys of run 0 (prefix) or 1 (own) that a workgroup's part of a segment has, and their pages.
+struct AttnKeys { uint32_t first, last, len; const int32_t* table; };
+__device__ __forceinline__ AttnKeys attn_keys(const AttentionArgs& a, const AttentionEntry& e, const AttnSegment& g, int run) {
+    const uint32_t len = run ? e.own : e.front, tile0 = run ? e.front_tiles : 0u;
+    const uint32_t first = (g.first > tile0 ? g.first - tile0 : 0u) * smelt_serving::kKeyTile, last = (g.last > tile0 ? g.last - tile0 : 0u) * smelt_serving::kKeyTile;
+    return AttnKeys{first, last < len ? last : len, len, run ? a.page_table + (size_t)e.sequence * a.pages_per_sequence : a.prefix_table};
+}
+
+// the lane, for code that seldom runs: nothing of it is worked out ahead and held in registers through the key loops
+__device__ __forceinline__ uint32_t attn_cold_lane() {
+    uint32_t lane = threadIdx.x % kWave;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// Whether rows that came out as NaN are to be formed again: among the part's values one is not finite that a row of the tile does not see, or
+// one is an infinity (which a probability that rounds to zero makes a NaN).  seen(run) tells what all of the rows see; the wave
+// looks at every `waves`-th group of keys, 16 bytes a lane and eight loads under way.
+template <class ActT, int D, class Seen>
+__device__ __forceinline__ bool attn_again(const AttentionArgs& a, const AttentionEntry& e, const AttnSegment& g, uint32_t wave, uint32_t waves, Seen seen) {
+    constexpr uint32_t U = 8, kKeys = 512 / D, kInfinity = ActT::kIsF16 ? 0x7C00u : 0x7F80u;
+    const uint32_t lane = attn_cold_lane();
+    bool found = false;
 #pragma unroll 1
     for (int run = 0; run < 2; ++run) {
-        const uint32_t len = run ? e.own : e.front, tile0 = run ? e.front_tiles : 0u;
-        const uint32_t first = (g.first > tile0 ? g.first - tile0 : 0u) * smelt_serving::kKeyTile;
-        uint32_t last = (g.last > tile0 ? g.last - tile0 : 0u) * smelt_serving::kKeyTile;
-        last = last < len ? last : len;
-        const scalar_table table = as_scalar(run ? a.page_table + (size_t)e.sequence * a.pages_per_sequence : a.prefix_table);
-        const AttnBounds b = bounds(run ? (int32_t)e.prefix : 0, (int32_t)len);
+        const AttnKeys part = attn_keys(a, e, g, run);
+        const AttnRun u = seen(run);
 #pragma unroll 1
-        for (uint32_t key = first; key < last; ++key) {
-            const uint32_t page = (uint32_t)table[__builtin_amdgcn_readfirstlane(key >> a.page_shift)], off = key & ((1u << a.page_shift) - 1u);
-            if (page >= a.pages) continue;
-            const size_t at = (((size_t)page * a.kv_heads + g.kv_head) * D) << a.page_shift;
-            use((int32_t)key >= b.lo && (int32_t)key < b.hi, a.k_cache + at + off * 8, a.v_cache + at + off * D);
+        for (uint32_t base = part.first + wave * kKeys * U; base < part.last; base += waves * kKeys * U) {
+            uint32_t page[U];
+            uint4_t v[U];
+#pragma unroll
+            for (uint32_t k = 0; k < U; ++k) {
+                const uint32_t key = base + k * kKeys + lane / (D / 8);
+                page[k] = (uint32_t)part.table[(key < part.last ? key : part.last - 1) >> a.page_shift];
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < U; ++k) {
+                const uint32_t key = base + k * kKeys + lane / (D / 8), off = (key < part.last ? key : part.last - 1) & ((1u << a.page_shift) - 1u);
+                const size_t at = (((size_t)(page[k] < a.pages ? page[k] : 0u) * a.kv_heads + g.kv_head) * D) << a.page_shift;
+                v[k] = *reinterpret_cast<const uint4_t*>(a.v_cache + at + off * D + (lane % (D / 8)) * 8);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < U; ++k) {
+                const int32_t key = (int32_t)(base + k * kKeys + lane / (D / 8));
+                const bool hidden = key < u.all_lo || key >= u.all_hi;
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t size = (v[k][i / 2] >> (16 * (i & 1))) & 0x7FFFu;
+                    odd = odd || size == kInfinity || (hidden && size > kInfinity);
+                }
+                found = found || (odd && key < (int32_t)part.last && page[k] < a.pages);
+            }
         }
+    }
+    return __any(found);
+}
+
+// Forms row r of the tile (a token's head, at its position, of the given maximum and sum) over the part's keys that it sees and puts it where
+// the segment's rows go, by a wave: a key a lane for the scores, D / 64 values a lane for the output.
+template <class ActT, int D>
+__device__ __forceinline__ void attn_form_row(const AttentionArgs& a, const AttentionEntry& e, const AttnSegment& g, uint32_t r, uint32_t token, uint32_t head, int32_t position,
+                                              float m, float sum, float c) {
+    constexpr uint32_t E = D / 64, U = 8;
+    const uint32_t lane = attn_cold_lane(), mask = (1u << a.page_shift) - 1u;
+    const float shift = m == -__builtin_inff() ? 0.0f : -m * c;
+    const uint16_t* row = a.q + (size_t)token * a.q_stride + (size_t)head * D + lane * E;
+    int q[E];
+    float y[E];
+#pragma unroll
+    for (uint32_t n = 0; n < E; ++n) { q[n] = __builtin_bit_cast(int, ActT::widen((uint16_t)(row[n] ^ (uint16_t)a.flip_q))); y[n] = 0.0f; }
+#pragma unroll 1
+    for (int run = 0; run < 2; ++run) {
+        const AttnKeys part = attn_keys(a, e, g, run);
+        const AttnBounds b = attn_bounds(a, AttnRow{true, token, 0, position}, run ? (int32_t)e.prefix : 0, (int32_t)part.len);
+        const uint32_t first = __builtin_amdgcn_readfirstlane((int32_t)part.first > b.lo ? part.first : (uint32_t)b.lo);
+        const int32_t last = __builtin_amdgcn_readfirstlane((int32_t)part.last < b.hi ? (int32_t)part.last : b.hi);
+#pragma unroll 1
+        for (uint32_t base = first; (int32_t)base < last; base += kWave) {
+            const uint32_t key = (int32_t)(base + lane) < last ? base + lane : (uint32_t)last - 1, page = (uint32_t)part.table[key >> a.page_shift], off = key & mask;
+            const bool seen = (int32_t)(base + lane) < last && page < a.pages;
+            const size_t at = (((size_t)(page < a.pages ? page : 0u) * a.kv_heads + g.kv_head) * D) << a.page_shift, value = at + off * D;
+            const uint16_t* k = a.k_cache + at + off * 8;
+            float dot = 0.0f;
+#pragma unroll 8
+            for (uint32_t d = 0; d < D / 8; ++d) {
+                const uint4_t x = *reinterpret_cast<const uint4_t*>(k + (d << (a.page_shift + 3)));
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    dot = __builtin_fmaf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(q[i % E], d * (8 / E) + i / E)), ActT::widen((uint16_t)(x[i / 2] >> (16 * (i & 1)))), dot);
+            }
+            const int p = __builtin_bit_cast(int, attn_exp2(__builtin_fmaf(dot, c, shift)));
+            const unsigned long long who = __ballot(seen);
+#pragma unroll 1
+            for (uint32_t n = 0; n < (uint32_t)kWave && (int32_t)(base + n) < last; n += U) {
+                struct alignas(2 * E) Values { uint16_t x[E]; } v[U];
+#pragma unroll
+                for (uint32_t k2 = 0; k2 < U; ++k2) {
+                    const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(value >> 32), n + k2) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)value, n + k2);
+                    v[k2] = *reinterpret_cast<const Values*>(a.v_cache + from + lane * E);
+                }
+#pragma unroll
+                for (uint32_t k2 = 0; k2 < U; ++k2) {
+                    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(p, n + k2));
+#pragma unroll
+                    for (uint32_t i = 0; i < E; ++i) y[i] = (who >> (n + k2)) & 1u ? __builtin_fmaf(w, ActT::widen(v[k2].x[i]), y[i]) : y[i];
+                }
+            }
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const bool answer = g.whole && a.part == smelt_serving::kWholeSequences;
+    float* dst = (g.whole ? attn_whole_row(a, token, head, D) : attn_piece(a, g, D) + 2 * a.row_tile + r * D) + lane * E;
+#pragma unroll
+    for (uint32_t n = 0; n < E; ++n) {
+        if (answer) a.out[((size_t)token * a.heads + head) * D + lane * E + n] = ActT::narrow(y[n] * inv);
+        else dst[n] = y[n];
     }
 }
 // maximum and sum over a lane's row of the streaming kernel: lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -481,6 +582,7 @@ struct AttnShared {
     float o[4][16 * RT][D + 4];      // (four floats of padding: neighbouring rows' 16-byte stores lie on different banks)
     float m[4][16 * RT], l[4][16 * RT];
     int32_t position[16 * RT];
+    uint32_t nan[2], again;          // rows that came out as NaN for no NaN score (segments take turns); whether they are formed again
 };
 
 // Few rows a sequence (decoding, drafted tokens): bound by the cache's bytes.  Four sequences of 50000 to 65536 keys, heads of 256: 183 us
@@ -506,6 +608,8 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
     const uint32_t unit_end = work.parts ? unit + 1 : smelt_serving::attention_start(work.split, blockIdx.x + 1);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, quarter = lane >> 4, col = lane & 15;
     const AttnScale scale = attn_scale(a);
+    uint32_t turn = 0;
+    if (threadIdx.x == 0) sh.nan[0] = sh.again = 0;
 #pragma unroll 1
     while (unit < unit_end) {
         const AttentionEntry e = attn_entry(a, index);
@@ -659,6 +763,8 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
             }
         }
         __syncthreads();
+        turn ^= 1;
+        if (threadIdx.x == 0) sh.nan[turn] = 0;          // the next segment's: every wave has read it by now
         const uint32_t rows_live = e.tokens * a.group - row0 < R ? e.tokens * a.group - row0 : R;
         const bool begins = g.first == g.tiles.lo;
         if (begins && !g.whole) attn_note_cut(a, attn_cut(a, e, work.split, g));
@@ -678,21 +784,7 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
                 sum += f * sh.l[w][r];
             }
             const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
-            if (__builtin_expect(sum == sum && (y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w), 0)) {
-                const uint16_t* q = a.q + (size_t)token * a.q_stride + (size_t)head * D;
-                const float shift = top == -__builtin_inff() ? 0.0f : -top * scale.c;
-                y = float4_t{0, 0, 0, 0};
-                attn_each_key<D>(a, e, g, [&](int32_t base, int32_t len) { return attn_bounds(a, AttnRow{true, token, 0, sh.position[r]}, base, len); },
-                                 [&](bool sees, const uint16_t* k, const uint16_t* v) {
-                    float dot = 0.0f;
-#pragma unroll 1
-                    for (uint32_t n = 0; n < D; ++n)
-                        dot = __builtin_fmaf(ActT::widen((uint16_t)(q[n] ^ (uint16_t)a.flip_q)), ActT::widen(k[((n / 8) << (a.page_shift + 3)) + n % 8]), dot);
-                    const float p = attn_exp2(__builtin_fmaf(dot, scale.c, shift));
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) y[n] = sees ? __builtin_fmaf(p, ActT::widen(v[d + n]), y[n]) : y[n];
-                });
-            }
+            if (__builtin_expect(sum == sum && (y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w), 0)) atomicOr(&sh.nan[turn ^ 1], 1u << r);
             float* dst = attn_whole_row(a, token, head, D);
             if (a.part != smelt_serving::kWholeSequences && begins && d == 0) attn_end_row(dst + D, a, work, g, r, top, sum);
             if (!g.whole) {
@@ -706,6 +798,34 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
             }
         }
         __syncthreads();
+        const uint32_t nans = __builtin_amdgcn_readfirstlane(sh.nan[turn ^ 1]);
+        if (__builtin_expect(nans != 0, 0)) {
+            const bool again = attn_again<ActT, D>(a, e, g, wave, 4, [&](int run) {
+                AttnBounds b[RT];
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    b[t] = attn_bounds(a, AttnRow{16 * t + col < rows_live, 0, 0, sh.position[16 * t + col]}, run ? (int32_t)e.prefix : 0, (int32_t)(run ? e.own : e.front));
+                return attn_run(a, e, run, row0, R, b, RT);
+            });
+            if (again && lane == 0) sh.again = 1;
+            __syncthreads();
+            if (sh.again) {
+                uint32_t nth = 0;
+#pragma unroll 1
+                for (uint32_t set = nans; set; set &= set - 1, ++nth) {
+                    if (nth % 4 != wave) continue;
+                    const uint32_t r = __builtin_ctz(set), i = (row0 + r) / a.group;
+                    float top = sh.m[0][r], sum = 0.0f;
+#pragma unroll
+                    for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, sh.m[w][r]);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) sum += (top == -__builtin_inff() ? 1.0f : attn_exp2((sh.m[w][r] - top) * scale.c)) * sh.l[w][r];
+                    attn_form_row<ActT, D>(a, e, g, r, e.first_token + i, g.kv_head * a.group + (row0 + r) - i * a.group, sh.position[r], top, sum, scale.c);
+                }
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) sh.again = 0;
+        }
     }
 }
 
@@ -786,7 +906,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
         attn_clear<D>(acc);
         uint4_t qf[D / 16];
         attn_load_q<D / 16>(a, row, a.q + (size_t)row.token * a.q_stride + (size_t)(g.kv_head * a.group + row.head) * D + 8 * half, 16, qf);
-        const uint32_t page_bytes = (a.kv_heads * D * 2) << a.page_shift, head_bytes = (g.kv_head * D * 2) << a.page_shift;
+        const uint32_t page_bytes = (a.kv_heads * D * 2) << a.page_shift, head_bytes = __builtin_amdgcn_readfirstlane((g.kv_head * D * 2) << a.page_shift);
         const uint64_t k_base = (uint64_t)(uintptr_t)a.k_cache + head_bytes, v_base = (uint64_t)(uintptr_t)a.v_cache + head_bytes;
 #pragma unroll 1
         for (int run = 0; run < 2; ++run) {
@@ -950,8 +1070,6 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) nan = nan || acc.o[j][i] != acc.o[j][i];
         const unsigned long long nans = __ballot(nan && l == l && row.live);
-        const uint32_t again = (uint32_t)nans | (uint32_t)(nans >> 32);          // rows
-        const bool done = !((again >> (lane & 31)) & 1u);
         if (row.live) {
             const uint32_t r = wave * 32 + (lane & 31), head = g.kv_head * a.group + row.head;
             if (g.whole && a.part == smelt_serving::kWholeSequences) {
@@ -961,7 +1079,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                 for (int j = 0; j < D / 32; ++j)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
-                        if (done) *reinterpret_cast<uint2_t*>(out + 32 * j + 2 * i) = uint2_t{attn_pack2<ActT>(acc.o[j][i] * inv, acc.o[j][i + 1] * inv),
+                        *reinterpret_cast<uint2_t*>(out + 32 * j + 2 * i) = uint2_t{attn_pack2<ActT>(acc.o[j][i] * inv, acc.o[j][i + 1] * inv),
                                                                                    attn_pack2<ActT>(acc.o[j][i + 2] * inv, acc.o[j][i + 3] * inv)};
             } else {
                 float* whole = attn_whole_row(a, row.token, head, D);
@@ -974,37 +1092,21 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
                 for (int j = 0; j < D / 32; ++j)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
-                        if (done) *reinterpret_cast<float4_t*>(dst + 4 * half + 32 * j + 2 * i) = float4_t{acc.o[j][i], acc.o[j][i + 1], acc.o[j][i + 2], acc.o[j][i + 3]};
+                        *reinterpret_cast<float4_t*>(dst + 4 * half + 32 * j + 2 * i) = float4_t{acc.o[j][i], acc.o[j][i + 1], acc.o[j][i + 2], acc.o[j][i + 3]};
             }
         }
-        // (a lane takes D / 64 values of one row after the other here)
-        for (uint32_t set = again; set; set &= set - 1) {
-            constexpr int E = D / 64;
-            const int from = __builtin_ctz(set);
-            const uint32_t d = lane * E, r = wave * 32 + from, token = __builtin_amdgcn_readlane(row.token, from), head = g.kv_head * a.group + __builtin_amdgcn_readlane(row.head, from);
-            const int32_t position = __builtin_amdgcn_readlane(row.position, from);
-            const float m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, acc.m), from)), sum = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), from));
-            const float shift = m == -__builtin_inff() ? 0.0f : -m * scale.c;
-            float q[E], y[E];
-#pragma unroll
-            for (int n = 0; n < E; ++n) { q[n] = ActT::widen((uint16_t)(a.q[(size_t)token * a.q_stride + (size_t)head * D + d + n] ^ (uint16_t)a.flip_q)); y[n] = 0.0f; }
-            attn_each_key<D>(a, e, g, [&](int32_t base, int32_t len) { return attn_bounds(a, AttnRow{true, token, 0, position}, base, len); },
-                             [&](bool sees, const uint16_t* k, const uint16_t* v) {
-                float dot = 0.0f;
-#pragma unroll
-                for (int n = 0; n < E; ++n) dot = __builtin_fmaf(q[n], ActT::widen(k[((d / 8) << (a.page_shift + 3)) + d % 8 + n]), dot);
-#pragma unroll
-                for (int off = 32; off > 0; off >>= 1) dot += __shfl_xor(dot, off);
-                const float p = attn_exp2(__builtin_fmaf(dot, scale.c, shift));
-#pragma unroll
-                for (int n = 0; n < E; ++n) y[n] = sees ? __builtin_fmaf(p, ActT::widen(v[d + n]), y[n]) : y[n];
+        // (the other waves' rows see other keys, so each wave looks and forms for itself)
+        if (__builtin_expect(nans != 0, 0)) {
+            const bool again = attn_again<ActT, D>(a, e, g, 0, 1, [&](int run) {
+                const AttnBounds b = attn_bounds(a, row, run ? (int32_t)e.prefix : 0, (int32_t)(run ? e.own : e.front));
+                return attn_run(a, e, run, row0, 32, &b, 1);
             });
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-            for (int n = 0; n < E; ++n) {
-                if (g.whole && a.part == smelt_serving::kWholeSequences) a.out[((size_t)token * a.heads + head) * D + d + n] = ActT::narrow(y[n] * inv);
-                else if (g.whole) attn_whole_row(a, token, head, D)[d + n] = y[n];
-                else piece[2 * R + r * D + d + n] = y[n];
+#pragma unroll 1
+            for (uint32_t set = again ? (uint32_t)nans | (uint32_t)(nans >> 32) : 0u; set; set &= set - 1) {
+                const int from = __builtin_ctz(set);
+                attn_form_row<ActT, D>(a, e, g, wave * 32 + from, __builtin_amdgcn_readlane(row.token, from), g.kv_head * a.group + __builtin_amdgcn_readlane(row.head, from),
+                                       __builtin_amdgcn_readlane(row.position, from), __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, acc.m), from)),
+                                       __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), from)), scale.c);
             }
         }
     }

@@ -373,3 +373,62 @@ def test_rows_whose_scores_are_nan(ctx, dtype, dim, n, own, prefix, where):
     assert np.isnan(sr.wide(got[rows], dtype)).all()
     assert np.array_equal(got[n[0]:], before[n[0]:])
     assert took < 3 * clean + 50, f"{took:.0f} us, {clean:.0f} before"
+
+
+# decoding, drafts and a prompt behind a few thousand keys: NaN among the values of a key that all rows see
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,own,prefix", [([1, 1, 2], [3000, 40, 700], 0), ([5, 1, 2], [3000, 40, 700], 500), ([300, 70], [2500, 90], 0), ([300, 70], [2500, 90], 500)])
+@pytest.mark.parametrize("dims", ["all", "one"])
+def test_values_of_nan_that_all_rows_see(ctx, dtype, dim, n, own, prefix, dims):
+    """The rows that see them say so, in those values; everything else is as it was bit for bit, and the batch does not take tens of times
+    as long."""
+    c = Case(ctx, dtype, n, own, 8, 2, dim, 64, prefix=prefix, poison=False)
+    table = c.load()
+    clean = timed(c, table)
+    before = c.result().copy()
+    c.vb[c.table[0, 0], :, 2, (slice(None) if dims == "all" else 5)] = 0x7E00 if dtype == fx.F16 else 0x7FC0
+    table = c.load()
+    took = timed(c, table)
+    got = sr.wide(c.result(), dtype).reshape(-1, 8, dim)
+    hit = np.zeros(got.shape, bool)
+    hit[:n[0], :, (slice(None) if dims == "all" else 5)] = True
+    assert np.array_equal(np.isnan(got), hit)
+    assert np.array_equal(c.result().reshape(hit.shape)[~hit], before.reshape(hit.shape)[~hit])
+    assert took < 8 * clean + 500, f"{took:.0f} us, {clean:.0f} before"
+
+
+@TYPES
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 3, 60])
+@pytest.mark.parametrize("bad", [0x7C00, 0xFC00])
+def test_an_infinity_whose_probability_is_small(ctx, dtype, dim, n, bad):
+    """exp(-20) is no number of fp16 next to the others, but times an infinity it is one."""
+    c = Case(ctx, dtype, [n], [n + 80], 4, 2, dim, 16, scale=1.0, poison=False)
+    c.qb[:] = 0
+    c.qb[:, ::dim] = fx.to_bits(np.float32([1.0]), dtype)[0]
+    c.q = sr.wide(c.qb, dtype).reshape(-1, 4, dim)
+    c.kb[:] = 0
+    at = (c.table[0, 1], slice(None), 7)
+    c.kb[at][:, 0] = fx.to_bits(np.float32([-20.0]), dtype)[0]
+    c.vb[at][:, 9] = bad if dtype == fx.F16 else (0x7F80 | bad & 0x8000)
+    table = c.load()
+    ctx.interpret_decode(table)
+    ctx.wait()
+    check_where_finite(c, c.result())
+
+
+@TYPES
+@pytest.mark.parametrize("dim,n,own,prefix", [(128, [4, 2], [5000, 300], 0), (256, [3, 1], [4000, 90], 700), (64, [90, 40], [3000, 200], 0), (128, [60, 33], [2000, 200], 600)])
+def test_infinities_in_long_sequences(ctx, dtype, dim, n, own, prefix):
+    """Segments that are cut over several workgroups, some parts of which are formed again."""
+    c = Case(ctx, dtype, n, own, 8, 2, dim, 64, prefix=prefix, poison=False, seed=5)
+    bad_values(c, [[own[0] - 1, own[0] - 2, 1700], [own[1] - 1]], [0, 5, dim - 1])
+    table = c.load()
+    ctx.interpret_decode(table)
+    ctx.wait()
+    check_where_finite(c, c.result())
+    first = c.result().copy()
+    ctx.interpret_decode(table)
+    ctx.wait()
+    assert np.array_equal(first, c.result())
