@@ -212,7 +212,10 @@ int smelt_emit_view_gate_up_swiglu(smelt_emitter *e, int weights_slot, const Sme
  * (No counterpart in the reference's names: its attention, rope and sampling shaders are not mirrored here.)
  * Every value of a record but the first (`tokens` / `rows`, which resolves to seqLen when dynamic != 0) is fixed when it is
  * emitted; lengths, positions and page tables are data in bound slots, so a captured graph follows them.  The record's grid is
- * nominal.  The emitter runs the launch's own checks (all but the slots' sizes) and refuses what the launch would refuse.
+ * nominal.  The emitter runs the launch's own checks of shapes, strides and overlaps within a slot (with the workspace of a context)
+ * and refuses what they refuse.  What only the memory tells is left to the launch: whether a slot is large enough, whether an operand
+ * lies where its type needs it (keys, values: 16 bytes, attention's output and the frequency table: 8, 32-bit data: 4, other rows: 2), and
+ * whether two slots name the same bytes.
  *
  * Rotary positions.  A head's first rotary_dim values are rotated by position * table[i], pair i being (i, i + rotary_dim / 2), or
  * (2 i, 2 i + 1) when interleaved; the rest is copied.  cos and sin are multiplied by `amplitude`.  The table is

@@ -127,3 +127,38 @@ def test_steps_eager_and_replayed(dtype):
         ctx.graph_destroy(graph); ctx.graph_destroy(graph2)
     finally:
         ctx.close(); other.close()
+
+
+def test_operands_that_lie_between_their_types_places_are_refused_at_launch():
+    """The emitter knows no addresses: it takes every offset, the launch refuses those that no load of the operand's type can take."""
+    ctx = rt.Context()
+    try:
+        for slot in range(1, 12):
+            ctx.alloc(slot, 1 << 16)
+        base = {
+            "rope": dict(x=B(1), y=B(2), positions=B(3), table=B(4)),
+            "paged_kv_append": dict(k=B(1), v=B(2), positions=B(3), slots=B(4), table=B(5), k_cache=B(6), v_cache=B(7), q=B(8), q_out=B(9)),
+            "paged_attention": dict(q=B(1), k_cache=B(2), v_cache=B(3), page_table=B(4), kv_lens=B(5), offsets=B(6), out=B(7), prefix_table=B(8), prefix_len=B(9)),
+            "verify_drafts": dict(target=B(1), draft=B(2), draft_tokens=B(3), offsets=B(4), u_accept=B(5), u_sample=B(6), temperature=B(7), tokens=B(8), counts=B(9))}
+        rest = {
+            "rope": dict(tokens=2, heads=2, head_dim=64, rotary_dim=64),
+            "paged_kv_append": dict(tokens=2, kv_heads=1, head_dim=64, rotary_dim=64, page_size=16, pages=2, q_heads=2),
+            "paged_attention": dict(tokens=2, sequences=1, heads=2, kv_heads=1, head_dim=64, page_size=16, pages=2, pages_per_sequence=2, scale=0.1, prefix_pages=1),
+            "verify_drafts": dict(rows=2, sequences=1, vocab=100)}
+        needs = dict(k_cache=16, v_cache=16, out=8, table=8, x=2, y=2, k=2, v=2, q=2, q_out=2, target=2, draft=2)      # (4 where it is not said)
+        for op, operands in base.items():
+            def go(**kw):
+                em = cc.Emitter()
+                getattr(em, op)(**{**operands, **rest[op], **kw})
+                return ctx.interpret_decode(em.table_for(ctx))
+
+            assert go() >= 1
+            for name, b in operands.items():
+                align = needs.get(name, 4)
+                for off in {align // 2, align - 1} - {0}:
+                    with pytest.raises(rt.SmeltHipError, match="aligned"):
+                        go(**{name: B(b.slot, off)})
+                assert go(**{name: B(b.slot, 2 * align)}) >= 1
+        ctx.wait()
+    finally:
+        ctx.close()
