@@ -991,7 +991,6 @@ const Pipeline* pipeline_for(smelt_hip_context* ctx, uint32_t index) {
 int encode_serving(smelt_hip_context* ctx, const Pipeline& p, const Launch& L, const SplitKWorkspace& ws) {
     ServingDevice dev;
     dev.compute_units = (uint32_t)std::max(1, ctx->props.multiProcessorCount);
-    dev.lds_limit = ctx->lds_limit;
     dev.workspace = ws.partial;
     dev.workspace_bytes = ws.partial_bytes;
     ServingPlan plan;

@@ -187,7 +187,7 @@ int Planner::rope() {
     if (a.tokens == 0) return 0;
     const uint32_t half = a.rot / 2;
     uint32_t q_heads = 0, kv_heads = 0, page = 0;
-    a.positions = P<int32_t>(append ? 2 : 2);
+    a.positions = P<int32_t>(2);
     if (!append) {
         q_heads = U(o + 1);
         a.amplitude = F(o + 4);

@@ -35,7 +35,6 @@ struct ServingStep {
 
 struct ServingDevice {
     uint32_t compute_units = 256;
-    size_t lds_limit = 65536;
     void* workspace = nullptr;
     size_t workspace_bytes = 0;
 };
