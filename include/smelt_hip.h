@@ -212,8 +212,8 @@ int smelt_hip_set_cache_seq_capacity(smelt_hip_context *ctx, uint32_t capacity);
 /* loadDispatchTable size check: SmeltRuntime.swift:6322-6350 (size % 360 == 0). */
 int smelt_hip_dispatch_table_count(size_t table_bytes, size_t *out_count);
 
-/* emitDecodeDispatchRecord: SmeltRuntime.swift:3187-3247.  Returns 1 if a kernel was
- * launched, 0 if the record was a swap / skipped, negative on error. */
+/* emitDecodeDispatchRecord: SmeltRuntime.swift:3187-3247.  Returns the number of kernels
+ * launched (1 for most records), 0 if the record was a swap, skipped or of no rows, negative on error. */
 int smelt_hip_encode_decode_record(smelt_hip_context *ctx, const SmeltDispatchRecord *rec,
                                    int cur, int alt, int32_t position);
 /* emitDispatchRecord: SmeltRuntime.swift:5990-6054 (minSeqLen guard, offset kinds 0-4, dynamic

@@ -291,7 +291,9 @@ int smelt_emit_paged_attention(smelt_emitter *e, const SmeltPagedCache *cache, S
  * temperature <= 0 (or not a number): a draft is taken while it is the row's largest logit (lowest token of equal ones), and
  * that token is drawn.  A draft outside the vocabulary is refused; a NaN logit counts as -inf, +inf as the largest finite number; a row
  * without any weight draws -1.  tokens[row]: the taken drafts, the drawn token, then -1; counts[s]: taken drafts.  Rows from
- * offsets[sequences] on are left as they were; a sequence without rows counts 0.  At most 65535 rows and sequences. */
+ * offsets[sequences] on are left as they were; a sequence without rows counts 0 (but a record of no rows at all launches nothing).  Whether a
+ * draft is taken is decided from 32-bit sums, which can turn it where u_accept lies within a few 1e-7 of p / q; what is drawn, from 64-bit ones.
+ * At most 65535 rows and sequences. */
 int smelt_emit_verify_drafts(smelt_emitter *e, SmeltBinding target, const SmeltBinding *draft,
                              SmeltBinding draft_tokens, SmeltBinding offsets, SmeltBinding u_accept,
                              SmeltBinding u_sample, SmeltBinding temperature, SmeltBinding tokens,

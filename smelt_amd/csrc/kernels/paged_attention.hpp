@@ -586,8 +586,8 @@ struct AttnShared {
 };
 
 // Few rows a sequence (decoding, drafted tokens): bound by the cache's bytes.  Four sequences of 50000 to 65536 keys, heads of 256: 183 us
-// with the join's 8 (947 MB, 5.2 TB/s, a copy reaches 5.1); the own keys of 64 sequences of 17 to 1024: 32 us (136 MB, 4.3 TB/s);
-// one token behind 1000 keys: 9 us, of which 4 pass before its first key.  A workgroup takes a run of units and works
+// with the join's 8 (947 MB, 5.2 TB/s, a copy reaches 5.1); the own keys of 64 sequences of 17 to 1024: 32 us in a run of launches
+// (136 MB, 4.3 TB/s), 39 by themselves; one token behind 1000 keys: 9 us, of which 4 pass before its first key.  A workgroup takes a run of units and works
 // through the segments it crosses, its four waves on every fourth key tile, straight from the cache.  Here the products are
 // v_mfma_f32_16x16x32 (lane l: row l % 16, quarter l / 16), one or two tiles of 16 rows against each key tile: with one, heads of
 // 256 leave room for two workgroups a compute unit, whose starts and ends hide behind each other.  V: a lane takes 8 neighbouring
@@ -837,12 +837,13 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
 // 4 keys x 16 values and get one value of 4 keys each), the 16-byte pieces of V rows placed so that the four keys of such a read lie
 // on different banks.
 //
-// Two prompt chunks of 1000 tokens behind 4000 keys, 32 heads of 128: 133 us, 780 TFLOP/s (a large library product reaches 1190).  A stage
-// takes about 4450 cycles a SIMD: its two waves' matrix instructions fill 2100 of them and their vector instructions (24 cycles a score and
+// Two prompt chunks of 900 and 1024 tokens behind up to 4000 keys, 32 heads of 128: 138 us with the join's 5, 750 TFLOP/s (a large library
+// product reaches 1190); 160 us by itself.  The matrix cores are busy for 31 % of the launch: its 248 segments have 105 key tiles on
+// average and 127 at most, and what is not in the stages is their start and end.  A stage takes about 4450 cycles a SIMD: its two waves' matrix instructions fill 2100 of them and their vector instructions (24 cycles a score and
 // lane) 1500; the barrier keeps both in the same phase for the rest.  Heads of 256 have one wave a SIMD, 1.5 us a tile against 0.5 of matrix
 // instructions: a wave issues one instruction every four cycles, so every scalar one counts.  With the turns written out as the matrix
 // instructions' shadows (scores of the next tile beside this one's probabilities; four waves of 64 rows for heads of 128) they took 34
-// us against 34.5 here for a prefix of 8192 against 384 rows, and the prompt chunks 185 us against 137.
+// us against 34.5 here for a prefix of 8192 against 384 rows, and the prompt chunks 185 us against 138.
 typedef short attn_short4_t __attribute__((ext_vector_type(4)));
 constexpr int kAttnBuffers = 4;
 

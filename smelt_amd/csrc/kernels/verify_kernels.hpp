@@ -10,10 +10,11 @@
 // refused draft; (4) the place of u in the running sum.  Sums that decide which token is drawn are 64-bit, from 64-bit
 // exponentials: with a 248320-entry vocabulary neighbouring places in the running sum are 4e-6 apart and closer, and a 32-bit
 // exponential is already off by 6e-8 of each weight.  The first launch's 32-bit exponentials only meet the accept test, which they can
-// turn when u falls within about 1e-7 of the ratio.  Sums are added in a fixed order: the same inputs give the same tokens.
+// turn when u falls within a few 1e-7 of the ratio.  Sums are added in a fixed order: the same inputs give the same tokens.
 // 64 sequences of 1 to 8 rows, 248320 logits: 105 us (254 MB, 50 us at a copy's rate): launch 1 takes 44 us (5.8 TB/s), 2 and 3 30 and
-// 22 us (the chosen rows' 64-bit exponentials: twenty 64-bit instructions a logit, about 14 us each), 4 takes 12.  One sequence: 26 us, four
-// launches of two or three dependent loads each.
+// 23 us (the chosen rows' 64-bit exponentials: twenty 64-bit instructions a logit, about 14 us each), 4 takes 12.  One sequence: 25 us, four
+// launches of two or three dependent loads each.  Rows that do not lie at whole 16 bytes (a stride that is no multiple of 8) are read two
+// bytes at a time: the 64 sequences with a vocabulary of 248319 216 us, one of 151935 31.
 #pragma once
 #include "common.hpp"
 #include "serving_args.hpp"
@@ -67,7 +68,8 @@ __device__ __forceinline__ float verify_weight32(float logit, float top, float r
     return __builtin_amdgcn_exp2f(__builtin_fmaxf((logit - top) * rate, -200.0f));
 }
 
-// ... in 64 bits: 2^a by its nearest whole power n and the Taylor series of 2^f, |f| <= 1/2, up to f^10 (the next term is below 2e-13).
+// ... in 64 bits: 2^a by its nearest whole power n and the Taylor series of 2^f, |f| <= 1/2, up to f^10 (the next term is at most 2.2e-13: a weight is off by
+// at most 3.0e-13 of itself, and neighbouring places of the running sum are about 4e-6 apart).
 // n is the low word of the sum with 1.5 * 2^52.  The coefficients sit in scalar registers, opaque to the compiler: it would otherwise
 // accumulate into a copy of each that it makes first, two instructions a term.
 struct VerifyExp {

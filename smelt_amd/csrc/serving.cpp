@@ -311,8 +311,8 @@ int Planner::attention() {
     // being read once against all rows; the tile kernel takes longer runs of rows, whose tiles read prefix and own keys alike.
     // 64 sequences of 6 rows, heads of 256, a prefix of 8192: 86 us, with tiles of 32 rows 93, with the tile kernel for prefix and own keys
     // 191.  24 sequences of 18 rows on average, heads of 128, a prefix of 2500: 67 us, with two tiles of 16 rows a sequence 69, with the
-    // tile kernel 60 (24 short sequences fill the machine once, and one launch is less than three; the lengths that would tell
-    // are not known here).
+    // tile kernel 60 (24 short sequences fill the machine once, and one launch is less than three).  The host knows the mean of the rows and not
+    // the lengths, so the rule does not see that case, nor a batch that mixes single tokens with a long prompt.
     const uint64_t rows = (uint64_t)a.tokens * a.group;
     const bool stream = rows <= (uint64_t)32 * a.sequences;
     const uint32_t tile_rows = dim == 256 ? 128 : 256;
@@ -338,8 +338,9 @@ int Planner::attention() {
             x.lead = kSegmentLead;
             x.least_units = x.lead + (r <= 32 ? 4 : 8);   // a key tile for each of four waves; stages to keep under way
         }
-        // a segment each from three quarters of the workgroups on: no parts to write and join (two prompt chunks of 1000 tokens behind
-        // 4000 keys, 240 segments: 137 us, in equal runs 150)
+        // a segment each from three quarters of the workgroups on: no parts to write and join (two prompt chunks of 900 and 1024 tokens behind
+        // up to 4000 keys, 248 segments: 138 us, in equal runs 150).  Not measured above the number of compute units, where the last
+        // round may be mostly empty.
         x.whole_from = r <= 32 ? ~0u : std::max(1u, dev.compute_units * 3 / 4);
     };
     char* ws = static_cast<char*>(dev.workspace);
