@@ -434,9 +434,9 @@ __device__ __forceinline__ void attn_clear(AttnAcc<D>& acc) {
 // sums are right: hidden scores are taken out before those).  That is rare and stands outside of the key loops: a search for such values
 // within them cost a fifth of their time.  Two kinds of rows are left as they are, since NaN is their answer.  A row whose sum is a NaN has
 // seen a score that is one (a NaN in q or in a key, or an infinite score).  And where every value that is not finite is a NaN that all of the
-// tile's rows see, it is theirs.  One sequence with a NaN among many: 64 that decode 83 us for a score and 87 for a value, as without
-// either; four with 50000 to 65536 keys 182 and 220 (without 182); two prompt chunks 150 and 380 (150), and 14600 for a value in the
-// last key, whose tile's other 255 rows are formed again; drafted tokens 66 and 66 (66), 330 for one in the last key.
+// tile's rows see, it is theirs.  One sequence with a NaN among many: 64 that decode 84 us for a score, as without, and 120 for a value
+// (formed again 13000); four with 50000 to 65536 keys 182 and 390 (71000); two prompt chunks 150 and 385 (82000), and 14600 for a value
+// in the last key, which the tile's rows before it do not see; drafted tokens 65 and 86, and 390 for one in the last key (11000).
 
 // The keys of run 0 (prefix) or 1 (own) that a workgroup's part of a segment has, and their pages.
 struct AttnKeys { uint32_t first, last, len; const int32_t* table; };
@@ -454,10 +454,10 @@ __device__ __forceinline__ uint32_t attn_cold_lane() {
 }
 
 // Whether rows that came out as NaN are to be formed again: among the part's values one is not finite that a row of the tile does not see, or
-// one is an infinity (which a probability that rounds to zero makes a NaN).  seen(run) tells what all of the rows see; the wave
-// looks at every `waves`-th group of keys, 16 bytes a lane and eight loads under way.
+// one is an infinity (which a probability that rounds to zero makes a NaN).  seen(run) tells what all of the rows see.  By a wave, 16 bytes a
+// lane and eight loads under way.
 template <class ActT, int D, class Seen>
-__device__ __forceinline__ bool attn_again(const AttentionArgs& a, const AttentionEntry& e, const AttnSegment& g, uint32_t wave, uint32_t waves, Seen seen) {
+__device__ __forceinline__ bool attn_again(const AttentionArgs& a, const AttentionEntry& e, const AttnSegment& g, Seen seen) {
     constexpr uint32_t U = 8, kKeys = 512 / D, kInfinity = ActT::kIsF16 ? 0x7C00u : 0x7F80u;
     const uint32_t lane = attn_cold_lane();
     bool found = false;
@@ -466,7 +466,7 @@ __device__ __forceinline__ bool attn_again(const AttentionArgs& a, const Attenti
         const AttnKeys part = attn_keys(a, e, g, run);
         const AttnRun u = seen(run);
 #pragma unroll 1
-        for (uint32_t base = part.first + wave * kKeys * U; base < part.last; base += waves * kKeys * U) {
+        for (uint32_t base = part.first; base < part.last; base += kKeys * U) {
             uint32_t page[U];
             uint4_t v[U];
 #pragma unroll
@@ -582,7 +582,6 @@ struct AttnShared {
     float o[4][16 * RT][D + 4];      // (four floats of padding: neighbouring rows' 16-byte stores lie on different banks)
     float m[4][16 * RT], l[4][16 * RT];
     int32_t position[16 * RT];
-    uint32_t nan[2], again;          // rows that came out as NaN for no NaN score (segments take turns); whether they are formed again
 };
 
 // Few rows a sequence (decoding, drafted tokens): bound by the cache's bytes.  Four sequences of 50000 to 65536 keys, heads of 256: 183 us
@@ -608,8 +607,6 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
     const uint32_t unit_end = work.parts ? unit + 1 : smelt_serving::attention_start(work.split, blockIdx.x + 1);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, quarter = lane >> 4, col = lane & 15;
     const AttnScale scale = attn_scale(a);
-    uint32_t turn = 0;
-    if (threadIdx.x == 0) sh.nan[0] = sh.again = 0;
 #pragma unroll 1
     while (unit < unit_end) {
         const AttentionEntry e = attn_entry(a, index);
@@ -763,12 +760,11 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
             }
         }
         __syncthreads();
-        turn ^= 1;
-        if (threadIdx.x == 0) sh.nan[turn] = 0;          // the next segment's: every wave has read it by now
         const uint32_t rows_live = e.tokens * a.group - row0 < R ? e.tokens * a.group - row0 : R;
         const bool begins = g.first == g.tiles.lo;
         if (begins && !g.whole) attn_note_cut(a, attn_cut(a, e, work.split, g));
         float* piece = attn_piece(a, g, D);
+        uint32_t nans = 0;                               // rows that came out as NaN for no NaN score (a row's values lie in one wave)
 #pragma unroll 1
         for (uint32_t item = threadIdx.x; item < rows_live * (D / 4); item += blockDim.x) {
             const uint32_t r = item / (D / 4), d = (item % (D / 4)) * 4;
@@ -784,7 +780,7 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
                 sum += f * sh.l[w][r];
             }
             const uint32_t i = (row0 + r) / a.group, token = e.first_token + i, head = g.kv_head * a.group + (row0 + r) - i * a.group;
-            if (__builtin_expect(sum == sum && (y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w), 0)) atomicOr(&sh.nan[turn ^ 1], 1u << r);
+            if (sum == sum && (y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w)) nans |= 1u << r;
             float* dst = attn_whole_row(a, token, head, D);
             if (a.part != smelt_serving::kWholeSequences && begins && d == 0) attn_end_row(dst + D, a, work, g, r, top, sum);
             if (!g.whole) {
@@ -797,35 +793,26 @@ __device__ __forceinline__ void attn_stream(const AttentionArgs& a) {
                 *reinterpret_cast<uint2_t*>(a.out + ((size_t)token * a.heads + head) * D + d) = uint2_t{attn_pack2<ActT>(y.x * inv, y.y * inv), attn_pack2<ActT>(y.z * inv, y.w * inv)};
             }
         }
-        __syncthreads();
-        const uint32_t nans = __builtin_amdgcn_readfirstlane(sh.nan[turn ^ 1]);
-        if (__builtin_expect(nans != 0, 0)) {
-            const bool again = attn_again<ActT, D>(a, e, g, wave, 4, [&](int run) {
+        if (__builtin_expect(__any(nans != 0), 0) && attn_again<ActT, D>(a, e, g, [&](int run) {
                 AttnBounds b[RT];
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
                     b[t] = attn_bounds(a, AttnRow{16 * t + col < rows_live, 0, 0, sh.position[16 * t + col]}, run ? (int32_t)e.prefix : 0, (int32_t)(run ? e.own : e.front));
                 return attn_run(a, e, run, row0, R, b, RT);
-            });
-            if (again && lane == 0) sh.again = 1;
-            __syncthreads();
-            if (sh.again) {
-                uint32_t nth = 0;
+            })) {
 #pragma unroll 1
-                for (uint32_t set = nans; set; set &= set - 1, ++nth) {
-                    if (nth % 4 != wave) continue;
-                    const uint32_t r = __builtin_ctz(set), i = (row0 + r) / a.group;
-                    float top = sh.m[0][r], sum = 0.0f;
+            while (const unsigned long long who = __ballot(nans != 0)) {
+                const uint32_t r = __builtin_ctz(__builtin_amdgcn_readlane(nans, __builtin_ctzll(who))), i = (row0 + r) / a.group;
+                nans &= ~(1u << r);
+                float top = sh.m[0][r], sum = 0.0f;
 #pragma unroll
-                    for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, sh.m[w][r]);
+                for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, sh.m[w][r]);
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) sum += (top == -__builtin_inff() ? 1.0f : attn_exp2((sh.m[w][r] - top) * scale.c)) * sh.l[w][r];
-                    attn_form_row<ActT, D>(a, e, g, r, e.first_token + i, g.kv_head * a.group + (row0 + r) - i * a.group, sh.position[r], top, sum, scale.c);
-                }
+                for (int w = 0; w < 4; ++w) sum += (top == -__builtin_inff() ? 1.0f : attn_exp2((sh.m[w][r] - top) * scale.c)) * sh.l[w][r];
+                attn_form_row<ActT, D>(a, e, g, r, e.first_token + i, g.kv_head * a.group + (row0 + r) - i * a.group, sh.position[r], top, sum, scale.c);
             }
-            __syncthreads();
-            if (threadIdx.x == 0) sh.again = 0;
         }
+        __syncthreads();
     }
 }
 
@@ -1098,7 +1085,7 @@ __device__ __forceinline__ void attn_tiles(const AttentionArgs& a) {
         }
         // (the other waves' rows see other keys, so each wave looks and forms for itself)
         if (__builtin_expect(nans != 0, 0)) {
-            const bool again = attn_again<ActT, D>(a, e, g, 0, 1, [&](int run) {
+            const bool again = attn_again<ActT, D>(a, e, g, [&](int run) {
                 const AttnBounds b = attn_bounds(a, row, run ? (int32_t)e.prefix : 0, (int32_t)(run ? e.own : e.front));
                 return attn_run(a, e, run, row0, 32, &b, 1);
             });

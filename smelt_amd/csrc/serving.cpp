@@ -349,7 +349,7 @@ int Planner::attention() {
         // (as many as there can be segments, where each may take one)
         uint64_t grid = x.part == kPrefix ? (std::max<uint64_t>(segments(x), x.workgroups * x.rounds) + 7) / 8 * 8 : (r <= 32 ? x.workgroups : std::max<uint64_t>(segments(x), x.workgroups));
         grid = std::min<uint64_t>(grid, 0xFFFFFFFFull);       // (refused for its threads)
-        if (r <= 32) step(r == 16 ? 0 : 1, x, (uint32_t)grid, 1, 1, 256, (size_t)4 * r * (dim + 4) * 4 + 9 * r * 4 + 12);
+        if (r <= 32) step(r == 16 ? 0 : 1, x, (uint32_t)grid, 1, 1, 256, (size_t)4 * r * (dim + 4) * 4 + 9 * r * 4);
         else step(2, x, (uint32_t)grid, 1, 1, dim == 256 ? 256 : 512, (size_t)4 * (dim == 256 ? 1 : 2) * 2 * 32 * dim * 2);
     };
     // units are counted in 32 bits
